@@ -154,7 +154,8 @@ typedef struct MkStatus {
 } MkStatus;
 
 /* sizeof() of the structs above as this library was compiled (0 MkModelDesc,
- * 1 MkLaunchInfo, 2 MkStatus, 3 MkNvfp4Matrix); lets a foreign-language binding
+ * 1 MkLaunchInfo, 2 MkStatus, 3 MkNvfp4Matrix, 4 MkPagedCache, 5 MkPagedBatch,
+ * 6 MkPagedAppend, 7 MkPagedAttention); lets a foreign-language binding
  * verify its own struct layout.  No counterpart in the reference. */
 int mk_abi_sizeof(int32_t which);
 
@@ -492,6 +493,92 @@ int mk_fp4_chain_prepare(const MkFp4ChainOperand *operands, int32_t length, int3
 int mk_fp4_chain_run(void *handle, void *stream);
 int mk_fp4_chain_status(void *handle, void *stream);
 void mk_fp4_chain_destroy(void *handle);
+
+/*
+ * Paged KV cache (no counterpart in the reference, whose caches are one dense
+ * slab per model, megakernels/llama.py:552-574).  Pages of `page_size` positions
+ * are handed to sequences through a page table; a page holds bf16, or E4M3 codes
+ * with one fp32 scale per page and KV head (value = code x scale).
+ *
+ * k_pages / v_pages: element (page, head, slot, d) at
+ *   page * page_stride + head * head_stride + slot * slot_stride + d   (elements; multiples of 16 bytes)
+ * head_dim 64 or 128, page_size 16, 32, 64 or 128.
+ */
+#define MK_CACHE_BF16 0
+#define MK_CACHE_E4M3 1
+#define MK_PAGED_MAX_SEQS 4096
+typedef struct MkPagedCache {
+    void *k_pages, *v_pages;       /* device */
+    float *k_scales, *v_scales;    /* device, [num_pages, num_kv_heads] (MK_CACHE_E4M3) */
+    int64_t page_stride, head_stride, slot_stride;
+    int32_t format;                /* MK_CACHE_* */
+    int32_t num_pages, page_size, num_kv_heads, head_dim;
+    int32_t reserved;
+} MkPagedCache;
+
+/*
+ * The sequences of a call.  Token rows of sequence b are cu_tokens[b] ..
+ * cu_tokens[b + 1] - 1, or tokens / seqs rows each when cu_tokens is NULL.  A
+ * negative page id means "no page": nothing is stored there, and its positions
+ * take no part in attention.  Page ids, positions and row offsets are device data
+ * and are checked there: what lies outside its tensor is left out and bit 1 (value
+ * 2) of *error_word is set; bit 0 if a bounded wait ran out.  Sequences of one call
+ * do not share the pages that it stores into.
+ */
+typedef struct MkPagedBatch {
+    const int32_t *page_table;     /* device [seqs, max_pages], rows table_stride apart */
+    int64_t table_stride;
+    const int32_t *positions;      /* device [seqs]: append: position of the first new row (negative: idle sequence);
+                                    * attention: cached length, the new rows included */
+    const int32_t *cu_tokens;      /* device [seqs + 1] or NULL */
+    int32_t *error_word;           /* device, zeroed by the caller */
+    int32_t seqs, tokens, max_pages;
+    int32_t reserved;
+} MkPagedBatch;
+
+/*
+ * Rotary embedding of new query and key rows and the append of keys and values.
+ * Rows are bf16 [tokens, heads, head_dim] at any token and head pitch (elements,
+ * multiples of 8).  rope tables fp32 [rope_positions, rot_dim] (rot_dim a multiple
+ * of 16 up to head_dim; elements from rot_dim on pass unchanged; NULL: no rotation),
+ * pairs (2i, 2i+1), or (i, i + rot_dim/2) with half_layout.  Products are rounded
+ * separately in fp32, results once.  q / q_out may be NULL; rows of idle sequences
+ * are left as they were.
+ *
+ * E4M3: a page's scale is 2^e, e the smallest integer in [-64, 120] with
+ * amax <= 448 * 2^e over the finite magnitudes of the page's rows; infinities
+ * saturate, NaN stays.  While a page holds rows its scale only grows, and the codes
+ * it holds are multiplied by the power of two; the first row of a page starts afresh.
+ */
+typedef struct MkPagedAppend {
+    const void *q, *k, *v;
+    void *q_out;                   /* bf16 [tokens, num_q_heads, head_dim]; may be q itself where q is that dense */
+    const float *rope_cos, *rope_sin;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int32_t num_q_heads, rot_dim, rope_positions, half_layout;
+} MkPagedAppend;
+int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *batch, const MkPagedAppend *args, void *stream);
+
+/*
+ * Causal attention of the new rows over the cache (which already holds their keys
+ * and values): row i of n sees positions 0 .. length - n + i.  out = softmax(scale q k) v in
+ * fp32, rounded once; rows that see nothing become zero, rows that belong to no
+ * sequence are left as they were.  Query heads are a multiple of the KV heads.
+ * The workspace (mk_paged_attention_workspace bytes for the same cache, batch sizes and
+ * device; 16-byte aligned, contents irrelevant) must not be shared by calls that may
+ * overlap in time.  Allocates nothing; may be captured in a CUDA graph.
+ */
+typedef struct MkPagedAttention {
+    const void *q;
+    void *out;                     /* bf16 [tokens, num_q_heads, head_dim] */
+    void *workspace;
+    int64_t workspace_bytes;
+    int64_t q_token_stride, q_head_stride;
+    int32_t num_q_heads;
+    float scale;
+} MkPagedAttention;
+int64_t mk_paged_attention_workspace(const MkPagedCache *cache, const MkPagedBatch *batch, int32_t num_q_heads);
+int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch *batch, const MkPagedAttention *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -32,6 +32,10 @@ MK_OPT_COOPERATIVE_LAUNCH = 5
 MK_WEIGHTS_BF16 = 0
 MK_WEIGHTS_NVFP4 = 1
 
+MK_CACHE_BF16 = 0
+MK_CACHE_E4M3 = 1
+MK_PAGED_MAX_SEQS = 4096
+
 EXPORTED_SYMBOLS = [
     "mk_last_error", "mk_create", "mk_set_schedule", "mk_step", "mk_query", "mk_status",
     "mk_set_wait_budget", "mk_status_detail", "mk_destroy", "mk_nvfp4_quantize", "mk_gemv", "mk_abi_sizeof", "mk_set_option",
@@ -42,6 +46,7 @@ EXPORTED_SYMBOLS = [
     "mk_batched_set_activation_scale",
     "mk_fp4_chain_prepare", "mk_fp4_chain_run", "mk_fp4_chain_status", "mk_fp4_chain_destroy",
     "mk_prefill_batched", "mk_batched_set_overlap", "mk_throughput_bind", "mk_throughput_set_schedule", "mk_step_throughput",
+    "mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace",
 ]
 
 
@@ -85,6 +90,39 @@ class MkThroughputBuffers(C.Structure):
         ("rms_rope_intermediates", C.c_void_p), ("rms_gate_intermediates", C.c_void_p),
         ("rms_lm_head_intermediates", C.c_void_p), ("post_ln_rope_q", C.c_void_p), ("attn_out", C.c_void_p),
         ("silu_out", C.c_void_p), ("barriers", C.c_void_p), ("barrier_cols", C.c_int32), ("batch_size", C.c_int32),
+    ]
+
+
+class MkPagedCache(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
+        ("format", C.c_int32), ("num_pages", C.c_int32), ("page_size", C.c_int32), ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class MkPagedBatch(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("positions", C.c_void_p), ("cu_tokens", C.c_void_p),
+        ("error_word", C.c_void_p), ("seqs", C.c_int32), ("tokens", C.c_int32), ("max_pages", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class MkPagedAppend(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("num_q_heads", C.c_int32), ("rot_dim", C.c_int32), ("rope_positions", C.c_int32), ("half_layout", C.c_int32),
+    ]
+
+
+class MkPagedAttention(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("num_q_heads", C.c_int32), ("scale", C.c_float),
     ]
 
 
@@ -158,13 +196,17 @@ def load() -> C.CDLL:
     lib.mk_throughput_bind.argtypes = [vp, C.POINTER(MkThroughputBuffers)]
     lib.mk_throughput_set_schedule.argtypes = [vp, vp, i32, i32]
     lib.mk_step_throughput.argtypes = [vp, i32, vp]
+    lib.mk_paged_append.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), C.POINTER(MkPagedAppend), vp]
+    lib.mk_paged_attention.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), C.POINTER(MkPagedAttention), vp]
+    lib.mk_paged_attention_workspace.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), i32]
+    lib.mk_paged_attention_workspace.restype = C.c_int64
     lib.mk_tp_init.argtypes = [vp, i32, i32, i32, vp]
     lib.mk_tp_connect.argtypes = [vp, vp, i32]
     lib.mk_abi_sizeof.argtypes = [i32]
     lib.mk_set_option.argtypes = [vp, i32, C.c_int64]
     for name in EXPORTED_SYMBOLS:
         if name not in ("mk_last_error", "mk_destroy", "mk_gemv_workspace_bytes", "mk_batched_destroy", "mk_fp4_chain_destroy",
-                        "mk_nvfp4_native_scale_bytes"):
+                        "mk_nvfp4_native_scale_bytes", "mk_paged_attention_workspace"):
             getattr(lib, name).restype = C.c_int
     lib.mk_gemv_workspace_bytes.restype = C.c_int64
     return lib

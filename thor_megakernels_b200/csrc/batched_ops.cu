@@ -24,60 +24,6 @@ namespace bo {
 constexpr int kNormThreads = 256;
 constexpr int kNormVecs = 8;   // float4 groups per thread: hidden sizes up to 8192
 
-// LinOut (batched_ops.cuh) is the result of a batched linear as its consumers
-// read it: bf16 y [batch, n], or the fp32 split-K partial sums [splits, batch, n],
-// which are added here in split order, scaled and rounded to bf16 once - the
-// value y would hold.
-__device__ __forceinline__ float lin_value(const LinOut &o, int b, int i) {
-    if (o.partials == nullptr) return __bfloat162float(o.y[(size_t)b * o.n + i]);
-    float total = 0.f;
-    for (int s = 0; s < o.splits; ++s) total += o.partials[((size_t)s * o.batch + b) * o.n + i];
-    return round_bf16(total * o.scale);
-}
-
-// Two / four consecutive elements (i even / a multiple of 4): vector loads, the splits'
-// loads independent of one another so that they are in flight together.
-__device__ __forceinline__ float2 lin_value2(const LinOut &o, int b, int i) {
-    if (o.partials == nullptr) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(o.y + (size_t)b * o.n + i));
-    float2 total = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < o.splits; ++s) {
-        const float2 v = *reinterpret_cast<const float2 *>(o.partials + ((size_t)s * o.batch + b) * o.n + i);
-        total.x += v.x; total.y += v.y;
-    }
-    return make_float2(round_bf16(total.x * o.scale), round_bf16(total.y * o.scale));
-}
-
-__device__ __forceinline__ float4 load_bf16x4(const bf16 *p) {
-    const uint2 raw = *reinterpret_cast<const uint2 *>(p);
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.x));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ void store_bf16x4(bf16 *p, const float4 &v) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    uint2 raw;
-    raw.x = *reinterpret_cast<const uint32_t *>(&a);
-    raw.y = *reinterpret_cast<const uint32_t *>(&b);
-    *reinterpret_cast<uint2 *>(p) = raw;
-}
-
-// sum of splits [s0, s1) for elements i..i+3, times the scale, rounded to bf16
-__device__ __forceinline__ float4 partial_sum4(const LinOut &o, int b, int i, int s0, int s1) {
-    float4 total = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-        const float4 v = *reinterpret_cast<const float4 *>(o.partials + ((size_t)s * o.batch + b) * o.n + i);
-        total.x += v.x; total.y += v.y; total.z += v.z; total.w += v.w;
-    }
-    return make_float4(round_bf16(total.x * o.scale), round_bf16(total.y * o.scale), round_bf16(total.z * o.scale),
-                       round_bf16(total.w * o.scale));
-}
-__device__ __forceinline__ float4 lin_value4(const LinOut &o, int b, int i) {
-    if (o.partials == nullptr) return load_bf16x4(o.y + (size_t)b * o.n + i);
-    return partial_sum4(o, b, i, 0, o.splits);
-}
-
 // hidden[b] = embed[token[b]]
 __global__ void embed_kernel(const bf16 *__restrict__ embed, const int *__restrict__ tokens, bf16 *__restrict__ hidden,
                              int hidden_size, int vocab, int *__restrict__ error) {

@@ -1965,6 +1965,10 @@ extern "C" int mk_abi_sizeof(int32_t which) {
     case 1: return (int)sizeof(MkLaunchInfo);
     case 2: return (int)sizeof(MkStatus);
     case 3: return (int)sizeof(MkNvfp4Matrix);
+    case 4: return (int)sizeof(MkPagedCache);
+    case 5: return (int)sizeof(MkPagedBatch);
+    case 6: return (int)sizeof(MkPagedAppend);
+    case 7: return (int)sizeof(MkPagedAttention);
     default: return -1;
     }
 }

@@ -1,0 +1,792 @@
+// Attention over a paged cache (bf16, or E4M3 with one scale per page and KV head): causal
+// queries at the end of every sequence, grouped query heads, any number of rows.
+//
+//   s[r, j] = scale * ks(page j) * q_r . k_j    for the positions j that row r sees
+//   out_r   = sum_j 2^(x_rj - m) vs(page j) v_j / sum_j 2^(x_rj - m),   x = s log2 e
+//
+// in one pass with a running maximum.  A row that sees nothing gives zeros.
+//
+// What bounds it.  With one or a few query tokens per sequence every cache byte is used for
+// a handful of rows: the kernel has to keep HBM busy and spend few instructions per byte.
+//   * Every warp is a worker of its own: it fills a private ring of shared-memory tiles (16 or
+//     32 positions of keys and values) with tiled TMA copies, one lane issuing, and no warp
+//     waits for another until the end of a segment.  The copies swizzle, so ldmatrix reads are
+//     free of bank conflicts, and read any page / head / slot pitch.  A page id outside the pool
+//     is outside the tensor map: the copy fills zeros.
+//   * Products are mma.sync.m16n8k16 with the CACHE as the 16-row operand (positions for the
+//     scores, head dimensions for the output) and the query rows as the 8 columns: a group of 4
+//     to 8 query heads fills the narrow side, so a cache element costs half the tensor
+//     instructions of the usual orientation.  The score fragment becomes the second product's
+//     operand through movmatrix (an 8x8 transpose inside the warp).  Both accumulators keep
+//     query rows in the same register positions: rescaling needs no shuffles.
+//   * E4M3 codes become f16 in registers (exact).  For keys, four consecutive codes of a row are
+//     one register; the columns' order inside a 16-wide step is then a permutation that the query
+//     fragment shares.  Values come through ldmatrix.trans on pairs of codes: one byte shuffle
+//     and two conversions give the fragment of even and odd columns.  Query rows enter as f16
+//     scaled by a power of two per row (exact for elements within 2^-31 of the row's largest).
+//   * The value scale joins the exponent: x + log2 vs is what the maximum runs over, so a weight
+//     that meets a page of large values is large in f16 and what is lost to its subnormals is
+//     small against the result.  The sum of the weights is taken in fp32 without that term.
+//   * A bf16 cache keeps bf16 operands; a weight enters as two terms (value and remainder).
+//
+// Work split.  Units of (row block, KV head, tile of 4 warp tiles) are dealt to the resident
+// CTAs in equal consecutive ranges: sequences of any lengths finish together, without knowing the
+// lengths on the host.  A segment that one CTA holds entirely is written at once; the others
+// leave (m, sum, output) in the workspace and a second kernel joins them in order.
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/b200_megakernel.h"
+#include "batched_ops.cuh"
+#include "paged_attention.cuh"
+#include "tma_host.cuh"
+
+namespace mk {
+
+void set_last_error(const char *msg);  // megakernel.cu
+
+namespace paged {
+
+template <int D, bool FP8>
+struct Tile {
+    static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
+    static constexpr int kPanelBytes = kRowBytes < 128 ? kRowBytes : 128;   // one swizzle row
+    static constexpr int kPanels = kRowBytes / kPanelBytes;
+    static constexpr int kTokens = kRowBytes == 256 ? 16 : 32;              // positions per warp tile
+    static constexpr int kBytes = kTokens * kRowBytes;                      // keys (and values)
+    static constexpr int kStages = kRowBytes == 64 ? 6 : 3;                 // 24 KiB per warp
+    static constexpr int kRing = kStages * 2 * kBytes;
+    static constexpr int kUnit = kWarps * kTokens;                          // positions per unit
+    static constexpr int kMmaTiles = kTokens / 16;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// four E4M3 codes -> two f16 pairs (low codes first)
+__device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_b16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int slot, int head, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
+}
+
+// Row blocks of this launch: NT tiles of 8 query rows.
+template <int D, bool FP8, int NT>
+__global__ void __launch_bounds__(kWarps * 32)
+decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
+    using T = Tile<D, FP8>;
+    constexpr int kRowsPerBlock = 8 * NT;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full[kWarps][T::kStages];
+    __shared__ float stat_m[kWarps][kRowsPerBlock], stat_l[kWarps][kRowsPerBlock];
+    __shared__ int scan_s[kWarps];
+    int *prefix = reinterpret_cast<int *>(smem + kWarps * T::kRing);   // [seqs + 1]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const Batch &bt = p.bt;
+    pdl_launch_dependents();
+    if (lane == 0)
+        for (int i = 0; i < T::kStages; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+    pdl_wait();
+
+    // units of the sequences before each one
+    {
+        const int per = (bt.seqs + kWarps * 32 - 1) / (kWarps * 32);
+        const int b0 = min((int)threadIdx.x * per, bt.seqs), b1 = min(b0 + per, bt.seqs);
+        int sum = 0;
+        for (int b = b0; b < b1; ++b) {
+            int first, count;
+            rows_of(bt, b, first, count);
+            const int units = count > p.max_count ? 0 : sequence_units(length_of(bt, b), count, p.group, kRowsPerBlock, T::kUnit, p.hkv);
+            prefix[b + 1] = units;
+            sum += units;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int off = 1; off < 32; off *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += v;
+        }
+        if (lane == 31) scan_s[warp] = incl;
+        __syncthreads();
+        int before = incl - sum;
+        for (int w = 0; w < warp; ++w) before += scan_s[w];
+        for (int b = b0; b < b1; ++b) {
+            before += prefix[b + 1];
+            prefix[b + 1] = before;
+        }
+        if (threadIdx.x == 0) prefix[0] = 0;
+        __syncthreads();
+    }
+    const int units = prefix[bt.seqs];
+    if (blockIdx.x == 0 && p.prefix_out)
+        for (int b = threadIdx.x; b <= bt.seqs; b += kWarps * 32) p.prefix_out[b] = prefix[b];
+    const int ctas = working_ctas(gridDim.x, units);
+    if ((int)blockIdx.x >= ctas) return;
+    int u = first_unit(blockIdx.x, ctas, units);
+    const int u_end = first_unit(blockIdx.x + 1, ctas, units);
+
+    uint8_t *ring = smem + warp * T::kRing;
+    const uint32_t ring_s = smem_addr(ring);
+    uint32_t stage = 0, parity = 0;
+    const int page_mask = (1 << bt.page_shift) - 1;
+    constexpr int kPagesPerTile = 2;   // at most: 32 positions over pages of 16
+
+    int b = 0;
+    while (u < u_end) {
+        // the segment that unit u lies in: sequence, row block, head, tile range
+        {
+            int lo = b, hi = bt.seqs - 1;   // last sequence with prefix <= u
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (prefix[mid] <= u) lo = mid;
+                else hi = mid - 1;
+            }
+            b = lo;
+        }
+        int first, count;
+        rows_of(bt, b, first, count);
+        const int length = length_of(bt, b);
+        int rest = u - prefix[b], rb = 0, tiles;
+        while (true) {
+            tiles = max(block_tiles(length, count, p.group, kRowsPerBlock, rb, T::kUnit), 1);
+            if (rest < tiles * p.hkv) break;
+            rest -= tiles * p.hkv;
+            ++rb;
+        }
+        const int head = rest / tiles, tile0 = rest % tiles;
+        const int tile1 = min(tiles, tile0 + (u_end - u));
+        const bool whole = tile0 == 0 && tile1 == tiles;
+        const int rows = min(kRowsPerBlock, count * p.group - rb * kRowsPerBlock);
+        const int last_token = min(((rb + 1) * kRowsPerBlock - 1) / p.group, count - 1);
+        const int seen = visible(length, count, last_token);                        // positions this block looks at
+        const int all_see = visible(length, count, rb * kRowsPerBlock / p.group);   // positions that every row sees
+        const int end = min(tile1 * T::kUnit, seen);
+        // this warp's tiles: positions from + i * kUnit
+        const int from = tile0 * T::kUnit + warp * T::kTokens;
+        const int n = end > from ? (end - from + T::kUnit - 1) / T::kUnit : 0;
+
+        // pages (and scales) of 32 tiles at a time, one tile per lane
+        const int *table = bt.table + b * bt.table_stride;
+        int page_cur[kPagesPerTile], page_next[kPagesPerTile];
+        float ks_cur[kPagesPerTile], vs_cur[kPagesPerTile], ks_next[kPagesPerTile], vs_next[kPagesPerTile];
+        auto load_pages = [&](int i0, int (&page)[kPagesPerTile]) {
+#pragma unroll
+            for (int h = 0; h < kPagesPerTile; ++h) {
+                const int pos = from + (i0 + lane) * T::kUnit + h * 16;
+                page[h] = -1;
+                if (i0 + lane < n && pos < end && (h * 16) < T::kTokens) {
+                    const int id = __ldg(table + (pos >> bt.page_shift));
+                    if (id >= bt.num_pages) atomicOr(bt.error, kErrorIndex);
+                    else page[h] = id;
+                }
+            }
+        };
+        auto load_scales = [&](const int (&page)[kPagesPerTile], float (&ks)[kPagesPerTile], float (&vs)[kPagesPerTile]) {
+            if constexpr (FP8) {
+#pragma unroll
+                for (int h = 0; h < kPagesPerTile; ++h) {
+                    ks[h] = 1.f;
+                    vs[h] = 0.f;
+                    if (page[h] >= 0) {
+                        const long long at = (long long)page[h] * p.hkv + head;
+                        ks[h] = __ldg(p.k_scales + at);
+                        vs[h] = log2f(fmaxf(__ldg(p.v_scales + at), 0x1p-100f));
+                    }
+                }
+            }
+        };
+        load_pages(0, page_cur);
+#pragma unroll
+        for (int h = 0; h < kPagesPerTile; ++h) page_next[h] = -1;
+
+        // fill of tile i into ring stage `st`
+        auto issue = [&](int i, uint32_t st, int cur0) {
+            int page[kPagesPerTile];
+            const bool next = i >= cur0 + 32;
+#pragma unroll
+            for (int h = 0; h < kPagesPerTile; ++h) page[h] = __shfl_sync(0xffffffffu, next ? page_next[h] : page_cur[h], i & 31);
+            if (lane == 0) {
+                const int pos = from + i * T::kUnit;
+                const uint32_t dst = ring_s + st * 2 * T::kBytes;
+                mbar_arrive_expect_tx(&full[warp][st], 2 * T::kBytes);
+                const int boxes = page_mask + 1 < T::kTokens ? T::kTokens / 16 : 1;   // pages of 16 come in two boxes
+                for (int h = 0; h < boxes; ++h) {
+#pragma unroll
+                    for (int panel = 0; panel < T::kPanels; ++panel) {
+                        const uint32_t at = dst + panel * T::kTokens * T::kPanelBytes + h * 16 * T::kPanelBytes;
+                        const int x = panel * T::kPanelBytes / (FP8 ? 1 : 2), slot = (pos + h * 16) & page_mask;
+                        tma_load_4d(at, &map_k, x, slot, head, page[h], &full[warp][st]);
+                        tma_load_4d(at + T::kBytes, &map_v, x, slot, head, page[h], &full[warp][st]);
+                    }
+                }
+            }
+        };
+        {
+            uint32_t st = stage;
+            for (int i = 0; i < min(n, T::kStages); ++i) {
+                issue(i, st, 0);
+                if (++st == T::kStages) st = 0;
+            }
+        }
+        load_scales(page_cur, ks_cur, vs_cur);
+
+        // query fragments: row g of tile nt, with the columns' order of the key fragments
+        uint32_t qf[D / 16][NT][2];
+        float q_scale[NT][2];   // of the columns 2t, 2t + 1 of a score fragment
+        int limit[NT][2];       // positions those rows see
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g, pair = rb * kRowsPerBlock + r;
+            const bool real = r < rows;
+            const bf16 *qp = p.q + (long long)(first + (real ? pair / p.group : 0)) * p.q_token +
+                             (long long)(head * p.group + (real ? pair % p.group : 0)) * p.q_head;
+            float unscale = 1.f;
+            if constexpr (FP8) {
+                uint32_t raw[D / 16][2];
+                float amax = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint2 v = real ? __ldg(reinterpret_cast<const uint2 *>(qp + 16 * ks + 4 * t)) : make_uint2(0u, 0u);
+                    raw[ks][0] = v.x;
+                    raw[ks][1] = v.y;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float a = fabsf(bf16_lo(raw[ks][i])), c = fabsf(bf16_hi(raw[ks][i]));
+                        if (a < INFINITY) amax = fmaxf(amax, a);
+                        if (c < INFINITY) amax = fmaxf(amax, c);
+                    }
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // 2^e with amax / 2^e in [2^14, 2^15); e stays where both it and its inverse are normal numbers
+                const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120);
+                const float factor = __uint_as_float((uint32_t)(127 - e) << 23);
+                unscale = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) qf[ks][nt][i] = pack_f16(bf16_lo(raw[ks][i]) * factor, bf16_hi(raw[ks][i]) * factor);
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        qf[ks][nt][i] = real ? __ldg(reinterpret_cast<const uint32_t *>(qp + 16 * ks + 2 * t + 8 * i)) : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                q_scale[nt][e] = p.scale_log2e * __shfl_sync(0xffffffffu, unscale, (2 * t + e) * 4);
+                const int r2 = nt * 8 + 2 * t + e;
+                limit[nt][e] = r2 < rows ? visible(length, count, (rb * kRowsPerBlock + r2) / p.group) : 0;
+            }
+        }
+
+        float m[NT][2], l[NT][2];
+        float o[D / 16][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) o[c][nt][0] = o[c][nt][1] = o[c][nt][2] = o[c][nt][3] = 0.f;
+        }
+
+        for (int i = 0; i < n; ++i) {
+            const int cur0 = i & ~31;
+            if ((i & 31) == 0 && i) {
+#pragma unroll
+                for (int h = 0; h < kPagesPerTile; ++h) { page_cur[h] = page_next[h]; ks_cur[h] = ks_next[h]; vs_cur[h] = vs_next[h]; }
+            }
+            if ((i & 31) == 12) load_pages(cur0 + 32, page_next);        // well before the first use, ...
+            if ((i & 31) == 24) load_scales(page_next, ks_next, vs_next);
+            // this tile's scales
+            float ks[T::kMmaTiles], vs[T::kMmaTiles];
+            bool absent = false;   // a position range without a page
+            const bool two = page_mask + 1 < T::kTokens;
+#pragma unroll
+            for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+                const int h = two ? mt : 0;
+                if constexpr (FP8) {
+                    const float k0 = __shfl_sync(0xffffffffu, ks_cur[0], i & 31), k1 = __shfl_sync(0xffffffffu, ks_cur[1], i & 31);
+                    const float v0 = __shfl_sync(0xffffffffu, vs_cur[0], i & 31), v1 = __shfl_sync(0xffffffffu, vs_cur[1], i & 31);
+                    ks[mt] = h ? k1 : k0;
+                    vs[mt] = h ? v1 : v0;
+                } else {
+                    ks[mt] = 1.f;
+                    vs[mt] = 0.f;
+                }
+            }
+            const int pg0 = __shfl_sync(0xffffffffu, page_cur[0], i & 31), pg1 = __shfl_sync(0xffffffffu, page_cur[1], i & 31);
+            absent = pg0 < 0 || (two && T::kMmaTiles > 1 && pg1 < 0);
+
+            const uint32_t kt = ring_s + stage * 2 * T::kBytes, vt = kt + T::kBytes;
+            const int pos0 = from + i * T::kUnit;
+            {
+                bool ok = mbar_try_wait(&full[warp][stage], parity);
+                if (!ok) {
+                    const long long began = clock64();
+                    while (!(ok = mbar_try_wait(&full[warp][stage], parity)))
+                        if (clock64() - began > kWaitCycles) break;
+                    if (!ok && lane == 0) atomicOr(bt.error, kErrorWait);
+                }
+                __syncwarp();
+            }
+
+            // scores [position][query row]
+            float sc[T::kMmaTiles][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < T::kMmaTiles; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+            const int mat = lane >> 3;
+            // address of 16-byte chunk c of position r in a tile
+            auto chunk_at = [&](uint32_t tile, int r, int c) {
+                if constexpr (T::kPanelBytes == 128)
+                    return tile + (c >> 3) * (T::kTokens * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                else
+                    return tile + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+            };
+#pragma unroll
+            for (int c2 = 0; c2 < T::kRowBytes / 32; ++c2) {
+#pragma unroll
+                for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+                    uint32_t kf[4];
+                    ldsm4(chunk_at(kt, mt * 16 + (mat & 1) * 8 + (lane & 7), 2 * c2 + (mat >> 1)), kf);
+                    if constexpr (FP8) {   // two 16-wide steps: chunk 2 c2 and chunk 2 c2 + 1
+                        uint32_t a[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) codes_to_f16(kf[j], a[2 * j], a[2 * j + 1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816<true>(sc[mt][nt], a[0], a[2], a[1], a[3], qf[2 * c2][nt][0], qf[2 * c2][nt][1]);
+                            mma16816<true>(sc[mt][nt], a[4], a[6], a[5], a[7], qf[2 * c2 + 1][nt][0], qf[2 * c2 + 1][nt][1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816<false>(sc[mt][nt], kf[0], kf[1], kf[2], kf[3], qf[c2][nt][0], qf[c2][nt][1]);
+                    }
+                }
+            }
+
+            // rows that look past their own last position, positions past the sequence, pages that are not there
+            const bool masked = absent || pos0 + T::kTokens > all_see;
+            if (masked) {
+                // A value that is not finite must not meet the zero weight of a row that does not see it: take it out
+                // of the tile, and give it to the rows that see it by hand.
+                uint32_t odd = 0;
+                for (int c = lane; c < T::kTokens * (T::kRowBytes / 16); c += 32) {
+                    const int r = c / (T::kRowBytes / 16), pos = pos0 + r;
+                    const uint32_t addr = chunk_at(vt, r, c % (T::kRowBytes / 16));
+                    if (pos >= length) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
+                    } else if (pos >= all_see) {
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) odd |= FP8 ? __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w[j] & 0x7f807f80u, 0x7f807f80u);
+                    }
+                }
+                __syncwarp();
+                if (__any_sync(0xffffffffu, odd != 0)) {
+                    for (int r = max(all_see - pos0, 0); r < min(T::kTokens, length - pos0); ++r) {
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {   // accumulator rows g and g + 8 of tile c
+                                const int d = FP8 ? 16 * c + 2 * g + half : 16 * c + 8 * half + g;
+                                const uint32_t at = chunk_at(vt, r, d * (FP8 ? 1 : 2) / 16) + d * (FP8 ? 1 : 2) % 16;
+                                uint32_t bits;
+                                if constexpr (FP8) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bits) : "r"(at));
+                                else asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bits) : "r"(at));
+                                const bool bad = FP8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u;
+                                if (bad) {
+                                    const float value = FP8 ? __int_as_float(0x7fffffff) : __uint_as_float(bits << 16);
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                        for (int e = 0; e < 2; ++e)
+                                            if (pos0 + r < limit[nt][e]) o[c][nt][2 * half + e] += value;
+                                }
+                            }
+                    }
+                    __syncwarp();
+                    for (int c = lane; c < T::kTokens * (T::kRowBytes / 4); c += 32) {
+                        const int r = c / (T::kRowBytes / 4), byte = c % (T::kRowBytes / 4) * 4;
+                        if (pos0 + r < all_see || pos0 + r >= length) continue;
+                        const uint32_t at = chunk_at(vt, r, byte / 16) + byte % 16;
+                        uint32_t w;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+                        w &= ~(FP8 ? __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w & 0x7f807f80u, 0x7f807f80u));
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy into this tile
+                __syncwarp();
+            }
+
+            // online softmax of rows 2t, 2t + 1 of every tile over this tile's positions
+            uint32_t pf[T::kMmaTiles][NT][2], pf_lo[T::kMmaTiles][NT][2];
+            bool rescale = false;
+            float corr[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+                        const float c = q_scale[nt][e] * ks[mt];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float x = FP8 ? fmaf(sc[mt][nt][2 * h + e], c, vs[mt]) : sc[mt][nt][2 * h + e] * c;
+                            if (masked) {
+                                const int pos = pos0 + mt * 16 + h * 8 + g;
+                                const bool there = (two && mt == 1 ? pg1 : pg0) >= 0;
+                                if (!(there && pos < limit[nt][e])) x = -INFINITY;
+                            }
+                            sc[mt][nt][2 * h + e] = x;
+                            mx = fmaxf(mx, x);
+                        }
+                    }
+#pragma unroll
+                    for (int off = 4; off < 32; off *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    const float mn = fmaxf(m[nt][e], mx);
+                    const float base = mn == -INFINITY ? 0.f : mn;
+                    corr[nt][e] = exp2_fast(m[nt][e] - base);
+                    rescale = rescale || mn != m[nt][e];
+                    m[nt][e] = mn;
+                    float add = 0.f;
+#pragma unroll
+                    for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+                        const float w0 = exp2_fast(sc[mt][nt][e] - base), w1 = exp2_fast(sc[mt][nt][2 + e] - base);
+                        sc[mt][nt][e] = w0;
+                        sc[mt][nt][2 + e] = w1;
+                        if constexpr (FP8) add = fmaf(w0 + w1, exp2_fast(-vs[mt]), add);
+                        else add += w0 + w1;
+                    }
+                    l[nt][e] = fmaf(l[nt][e], corr[nt][e], add);
+                }
+#pragma unroll
+                for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float w0 = sc[mt][nt][2 * h], w1 = sc[mt][nt][2 * h + 1];
+                        if constexpr (FP8) {
+                            pf[mt][nt][h] = transpose8(pack_f16(w0, w1));
+                        } else {
+                            const uint32_t hi = pack_b16(w0, w1);
+                            pf[mt][nt][h] = transpose8(hi);
+                            pf_lo[mt][nt][h] = transpose8(pack_b16(w0 - bf16_lo(hi), w1 - bf16_hi(hi)));
+                        }
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[c][nt][j] *= corr[nt][j & 1];
+            }
+
+            // output [dimension][query row] += values^T weights
+#pragma unroll
+            for (int mt = 0; mt < T::kMmaTiles; ++mt) {
+#pragma unroll
+                for (int c2 = 0; c2 < T::kRowBytes / 32; ++c2) {
+                    uint32_t vf[4];
+                    if constexpr (FP8) {
+                        ldsm4_trans(chunk_at(vt, mt * 16 + (mat & 1) * 8 + (lane & 7), 2 * c2 + (mat >> 1)), vf);
+                        uint32_t a[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) codes_to_f16(__byte_perm(vf[j], 0u, 0x3120), a[2 * j], a[2 * j + 1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816<true>(o[2 * c2][nt], a[0], a[1], a[2], a[3], pf[mt][nt][0], pf[mt][nt][1]);
+                            mma16816<true>(o[2 * c2 + 1][nt], a[4], a[5], a[6], a[7], pf[mt][nt][0], pf[mt][nt][1]);
+                        }
+                    } else {
+                        ldsm4_trans(chunk_at(vt, mt * 16 + (mat >> 1) * 8 + (lane & 7), 2 * c2 + (mat & 1)), vf);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816<false>(o[c2][nt], vf[0], vf[1], vf[2], vf[3], pf[mt][nt][0], pf[mt][nt][1]);
+                            mma16816<false>(o[c2][nt], vf[0], vf[1], vf[2], vf[3], pf_lo[mt][nt][0], pf_lo[mt][nt][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (i + T::kStages < n) issue(i + T::kStages, stage, cur0);
+            if (++stage == T::kStages) { stage = 0; parity ^= 1u; }
+        }
+
+        // the warps' states meet in shared memory (each warp's ring is idle now)
+        float *mine = reinterpret_cast<float *>(ring);   // [row][D]
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int off = 4; off < 32; off *= 2) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+                const int r = nt * 8 + 2 * t + e;
+                if (g == 0) {
+                    stat_m[warp][r] = m[nt][e];
+                    stat_l[warp][r] = l[nt][e];
+                }
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int d = FP8 ? 16 * c + 2 * g + half : 16 * c + 8 * half + g;
+                        mine[r * D + d] = o[c][nt][2 * half + e];
+                    }
+            }
+        }
+        __syncthreads();
+        // slot of the workspace: 0 continues a segment that an earlier CTA began, 1 begins one that a later CTA ends
+        float *part = p.partial + ((long long)blockIdx.x * 2 + (tile0 == 0 ? 1 : 0)) * kRowsPerBlock * (D + 2);
+        for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kWarps * 32) {
+            const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, stat_m[w][r]);
+            const float base = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2_fast(stat_m[w][r] - base);
+                L = fmaf(stat_l[w][r], f, L);
+                const float4 v = *reinterpret_cast<const float4 *>(smem + w * T::kRing + (r * D + d) * 4);
+                O.x = fmaf(v.x, f, O.x); O.y = fmaf(v.y, f, O.y); O.z = fmaf(v.z, f, O.z); O.w = fmaf(v.w, f, O.w);
+            }
+            if (whole) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                const int pair = rb * kRowsPerBlock + r;
+                bf16 *dst = p.out + ((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + d;
+                bo::store_bf16x4(dst, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
+            } else {
+                *reinterpret_cast<float2 *>(part + r * (D + 2) + d) = make_float2(O.x, O.y);
+                *reinterpret_cast<float2 *>(part + r * (D + 2) + d + 2) = make_float2(O.z, O.w);
+                if (d == 0) *reinterpret_cast<float2 *>(part + r * (D + 2) + D) = make_float2(M, L);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's plain writes, before the next copies into it
+        __syncthreads();
+        u += tile1 - tile0;
+    }
+}
+
+// Joins the parts of the segments that several CTAs shared: one CTA per (sequence, KV head), its
+// warps taking every eighth part, four columns per lane.  Weights 2^(m_part - max m), parts in order.
+template <int D>
+__global__ void __launch_bounds__(256)
+join_kernel(const AttentionParams p, int rows_per_block, int unit, int grid) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const Batch &bt = p.bt;
+    __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
+    const int b = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int u_seq = __ldg(p.prefix_out + b), units = __ldg(p.prefix_out + bt.seqs);
+    if (__ldg(p.prefix_out + b + 1) == u_seq) return;
+    const int ctas = working_ctas(grid, units);
+    int first, count;
+    rows_of(bt, b, first, count);
+    const int length = length_of(bt, b), blocks = block_count(count, p.group, rows_per_block);
+    int at = u_seq;
+    for (int rb = 0; rb < blocks; ++rb) {
+        const int tiles = max(block_tiles(length, count, p.group, rows_per_block, rb, unit), 1);
+        const int u0 = at + head * tiles, u1 = u0 + tiles;
+        at += tiles * p.hkv;
+        const int c0 = owner(u0, ctas, units), c1 = owner(u1 - 1, ctas, units);
+        if (c0 == c1) continue;   // written by its only CTA
+        const int rows = min(rows_per_block, count * p.group - rb * rows_per_block);
+        for (int r = 0; r < rows; ++r) {
+            float M = -INFINITY, L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto part_of = [&](int c) {
+                return p.partial + (((long long)c * 2 + (c == c0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
+            };
+            for (int c = c0 + warp; c <= c1; c += 8) {
+                const float2 ml = *reinterpret_cast<const float2 *>(part_of(c) + D);
+                M = fmaxf(M, ml.x);
+            }
+            const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+            for (int c = c0 + warp; c <= c1; c += 8) {
+                const float *src = part_of(c);
+                const float2 ml = *reinterpret_cast<const float2 *>(src + D);
+                const float f = exp2_fast(ml.x - base);
+                L = fmaf(ml.y, f, L);
+                if (4 * lane < D) {
+                    const float2 x = *reinterpret_cast<const float2 *>(src + 4 * lane), y = *reinterpret_cast<const float2 *>(src + 4 * lane + 2);
+                    O.x = fmaf(x.x, f, O.x); O.y = fmaf(x.y, f, O.y); O.z = fmaf(y.x, f, O.z); O.w = fmaf(y.y, f, O.w);
+                }
+            }
+            __syncthreads();
+            if (lane == 0) {
+                sum_m[warp] = M;
+                sum_l[warp] = L;
+            }
+            if (4 * lane < D) *reinterpret_cast<float4 *>(&sum_o[warp][4 * lane]) = O;
+            __syncthreads();
+            if ((int)threadIdx.x < D) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) top = fmaxf(top, sum_m[w]);
+                top = top == -INFINITY ? 0.f : top;
+                float total = 0.f, value = 0.f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    const float f = exp2_fast(sum_m[w] - top);
+                    total = fmaf(sum_l[w], f, total);
+                    value = fmaf(sum_o[w][threadIdx.x], f, value);
+                }
+                const int pair = rb * rows_per_block + r;
+                p.out[((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + threadIdx.x] =
+                    __float2bfloat16_rn(total == 0.f ? 0.f : value / total);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// Query rows that a sequence of this call can have at most, in tiles of 8, rounded up to 1, 2 or 4
+// tiles per row block (a block of more rows reads the cache once for all of them).
+static int row_tiles(const Batch &bt, int group, int max_count) {
+    const long long most = bt.cu ? (bt.tokens < max_count ? bt.tokens : max_count) : bt.per_seq;
+    const long long rows = most * group;
+    return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
+
+bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const int bytes = pool.fp8 ? 1 : 2;
+    const int panel = pool.head_dim * bytes < 128 ? pool.head_dim * bytes : 128;
+    const cuuint64_t dims[4] = {(cuuint64_t)pool.head_dim, (cuuint64_t)pool.page_size, (cuuint64_t)pool.kv_heads, (cuuint64_t)pool.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(pool.slot_stride * bytes), (cuuint64_t)(pool.head_stride * bytes),
+                                   (cuuint64_t)(pool.page_stride * bytes)};
+    const cuuint32_t box[4] = {(cuuint32_t)(panel / bytes), (cuuint32_t)box_tokens, 1, 1};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    return fn(map, pool.fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides,
+              box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, panel == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool FP8, int NT>
+static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
+    using T = Tile<D, FP8>;
+    CUtensorMap map_k, map_v;
+    const int box = pool.page_size < T::kTokens ? pool.page_size : T::kTokens;
+    if (!make_pool_map(&map_k, pool, pool.k, box) || !make_pool_map(&map_v, pool, pool.v, box)) {
+        set_last_error("mk_paged_attention: cuTensorMapEncodeTiled refused the cache (driver without tensor-map support?)");
+        return MK_ERR_UNSUPPORTED;
+    }
+    const size_t smem = 1024 + kWarps * T::kRing + (size_t)(p.bt.seqs + 1) * sizeof(int);
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<D, FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    const DecodeGrid grid = decode_grid(pool, p.bt, p.hq, p.max_count, sms);
+    e = launch_pdl(decode_kernel<D, FP8, NT>, dim3(grid.ctas), dim3(kWarps * 32), smem, st, map_k, map_v, p);
+    if (e == cudaSuccess && grid.split)
+        e = launch_pdl(join_kernel<D>, dim3(p.bt.seqs, p.hkv), dim3(256), 0, st, p, 8 * NT, T::kUnit, grid.ctas);
+    return (int)e;
+}
+
+template <int D, bool FP8>
+static int launch_decode_d(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
+    switch (row_tiles(p.bt, p.group, p.max_count)) {
+    case 1: return launch_decode_t<D, FP8, 1>(p, pool, sms, st);
+    case 2: return launch_decode_t<D, FP8, 2>(p, pool, sms, st);
+    default: return launch_decode_t<D, FP8, 4>(p, pool, sms, st);
+    }
+}
+
+DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count, int sms) {
+    const int row_bytes = pool.head_dim * (pool.fp8 ? 1 : 2);
+    const int unit = kWarps * (row_bytes == 256 ? 16 : 32);
+    const int group = hq / pool.kv_heads, rows = 8 * row_tiles(bt, group, max_count);
+    const long long tiles = (((long long)bt.max_pages << bt.page_shift) + unit - 1) / unit;
+    const long long blocks = bt.cu ? (long long)bt.tokens * group / rows + bt.seqs : (long long)bt.seqs * block_count(bt.per_seq, group, rows);
+    const long long most = blocks * pool.kv_heads * (tiles > 0 ? tiles : 1);
+    DecodeGrid g;
+    g.ctas = (int)(most < 2ll * sms ? most : 2ll * sms);   // two resident CTAs per SM
+    g.split = tiles > 1;
+    g.too_many = most > 0x7fffffffll;
+    g.partial_floats = g.split ? (long long)g.ctas * 2 * rows * (pool.head_dim + 2) : 0;
+    return g;
+}
+
+int launch_decode(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
+    if (pool.head_dim == 64)
+        return pool.fp8 ? launch_decode_d<64, true>(p, pool, sms, st) : launch_decode_d<64, false>(p, pool, sms, st);
+    return pool.fp8 ? launch_decode_d<128, true>(p, pool, sms, st) : launch_decode_d<128, false>(p, pool, sms, st);
+}
+
+static int max_count_of_decode() { return 0x7fffffff; }
+
+long long attention_workspace(const Batch &bt, const Pool &pool, int hq, int sms) {
+    const DecodeGrid g = decode_grid(pool, bt, hq, max_count_of_decode(), sms);
+    if (g.too_many) return -1;
+    return g.split ? 4ll * (((bt.seqs + 1 + 3) & ~3) + g.partial_floats) : 0;
+}
+
+int launch_attention(AttentionParams p, const Pool &pool, void *workspace, int sms, cudaStream_t st) {
+    p.max_count = max_count_of_decode();
+    p.prefix_out = reinterpret_cast<int *>(workspace);
+    p.partial = reinterpret_cast<float *>(workspace) + ((p.bt.seqs + 1 + 3) & ~3);
+    return launch_decode(p, pool, sms, st);
+}
+
+}  // namespace paged
+}  // namespace mk
