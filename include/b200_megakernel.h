@@ -506,7 +506,8 @@ void mk_fp4_chain_destroy(void *handle);
  */
 #define MK_CACHE_BF16 0
 #define MK_CACHE_E4M3 1
-#define MK_PAGED_MAX_SEQS 4096
+#define MK_PAGED_MAX_SEQS 4096            /* sequences per append */
+#define MK_PAGED_ATTENTION_MAX_SEQS 1024  /* and per attention call */
 typedef struct MkPagedCache {
     void *k_pages, *v_pages;       /* device */
     float *k_scales, *v_scales;    /* device, [num_pages, num_kv_heads] (MK_CACHE_E4M3) */

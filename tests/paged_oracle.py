@@ -64,8 +64,10 @@ def attention(q, k, v, table, lengths, cu, page, scale):
     return out, mag
 
 
-def attention_tolerance(ref, mag, fp8, positions, vmax):
-    """Result rounded to bf16 (2^-8); weights rounded to f16 (2^-11, and 2^-25 of the largest where that is less) for the 8-bit
-    cache, to two bf16 terms (2^-16) otherwise; scores and sums in fp32 (2^-14 is generous for up to 128 products and 2^14
-    positions)."""
-    return 2.0 ** -8 * ref.abs() + ((2.0 ** -11 if fp8 else 2.0 ** -16) + 2.0 ** -14) * mag + (positions * 2.0 ** -25 * vmax if fp8 else 0.0)
+def attention_tolerance(ref, mag, fp8, positions, vmax, many_rows=False):
+    """Result rounded to bf16 (2^-8).  Weights: f16 (2^-11, and 2^-25 of the largest where that is less) for the 8-bit cache; two
+    bf16 terms (2^-16) for a bf16 cache; one bf16 term where a sequence has more than 32 (token, head of the group) rows and the
+    large-tile kernel takes it: |sum w_j (1 + e_j) v_j - sum w_j v_j| <= max |e_j| sum w_j |v_j| = 2^-8 mag.  Scores and sums in fp32
+    (2^-14 is generous for up to 128 products and 2^14 positions)."""
+    weight = 2.0 ** -11 if fp8 else 2.0 ** -8 if many_rows else 2.0 ** -16
+    return 2.0 ** -8 * ref.abs() + (weight + 2.0 ** -14) * mag + (positions * 2.0 ** -25 * vmax if fp8 else 0.0)

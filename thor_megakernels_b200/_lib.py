@@ -35,6 +35,7 @@ MK_WEIGHTS_NVFP4 = 1
 MK_CACHE_BF16 = 0
 MK_CACHE_E4M3 = 1
 MK_PAGED_MAX_SEQS = 4096
+MK_PAGED_ATTENTION_MAX_SEQS = 1024
 
 EXPORTED_SYMBOLS = [
     "mk_last_error", "mk_create", "mk_set_schedule", "mk_step", "mk_query", "mk_status",

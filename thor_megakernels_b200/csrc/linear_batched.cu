@@ -51,6 +51,7 @@
 #include "../../include/b200_megakernel.h"
 #include "mk_device.cuh"
 #include "batched_ops.cuh"
+#include "tcgen05.cuh"
 #include "tma_host.cuh"
 
 namespace mk {
@@ -123,13 +124,6 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, i
         : "memory");
 }
 
-// Shared-memory matrix descriptor of a K-major tile whose rows are 128 bytes
-// (one swizzle row): start address, 8-row groups 1024 bytes apart, 128-byte swizzle.
-__device__ __forceinline__ uint64_t smem_desc_k_major_sw128(const void *tile) {
-    const uint64_t addr = smem_addr(tile);
-    return ((addr >> 4) & 0x3fffull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
 // kind::f16 instruction descriptor: bf16 x bf16 -> fp32, both operands K-major, M = 128.
 __device__ __forceinline__ uint32_t idesc_bf16(int n) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kSlabRows >> 4) << 24);
@@ -167,14 +161,6 @@ __device__ __forceinline__ void copy_scales_to_tmem(uint32_t taddr, const void *
     const uint64_t desc = ((addr >> 4) & 0x3fffull) | (8ull << 32) | (1ull << 46);
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-
-// Arrives on the barrier once every MMA issued so far by this thread has completed.
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // 32 lanes x 16 consecutive fp32 columns of tensor memory: thread i gets lane (base lane + i).
 __device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&v)[16]) {

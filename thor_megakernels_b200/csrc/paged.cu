@@ -25,7 +25,7 @@ static int refuse(int code, const char *who, const char *text) {
 static bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 // Pool and batch of a call, or an error code.
-static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, Pool &pool, Batch &bt, const char *who) {
+static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs, Pool &pool, Batch &bt, const char *who) {
     if (!c.k_pages || !c.v_pages || !b.page_table || !b.positions || !b.error_word)
         return refuse(MK_ERR_BAD_ARGUMENT, who, "null pointer");
     if (c.format != MK_CACHE_BF16 && c.format != MK_CACHE_E4M3) return refuse(MK_ERR_UNSUPPORTED, who, "unknown cache format");
@@ -36,7 +36,7 @@ static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, Pool &pool, 
         return refuse(MK_ERR_UNSUPPORTED, who, "page_size must be 16, 32, 64 or 128");
     if (c.num_pages < 1 || c.num_kv_heads < 1 || b.seqs < 1 || b.tokens < 1 || b.max_pages < 1)
         return refuse(MK_ERR_BAD_ARGUMENT, who, "empty cache or batch");
-    if (b.seqs > MK_PAGED_MAX_SEQS) return refuse(MK_ERR_UNSUPPORTED, who, "more sequences than one call takes");
+    if (b.seqs > max_seqs) return refuse(MK_ERR_UNSUPPORTED, who, "more sequences than one call takes");
     if (!b.cu_tokens && b.tokens % b.seqs) return refuse(MK_ERR_BAD_ARGUMENT, who, "rows do not divide evenly over the sequences");
     if (b.table_stride < b.max_pages && b.seqs > 1) return refuse(MK_ERR_BAD_ARGUMENT, who, "page table rows overlap");
     const int unit = fp8 ? 16 : 8;   // elements in 16 bytes
@@ -74,7 +74,7 @@ extern "C" int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *ba
     const char *who = "mk_paged_append";
     if (!cache || !batch || !a) return refuse(MK_ERR_BAD_ARGUMENT, who, "null argument");
     AppendParams p = {};
-    int code = read_cache(*cache, *batch, p.pool, p.bt, who);
+    int code = read_cache(*cache, *batch, MK_PAGED_MAX_SEQS, p.pool, p.bt, who);
     if (code) return code;
     if (bad_rows(a->k, a->k_token_stride, a->k_head_stride) || bad_rows(a->v, a->v_token_stride, a->v_head_stride))
         return refuse(MK_ERR_BAD_ARGUMENT, who, "key or value rows null or not on 16-byte boundaries");
@@ -104,7 +104,7 @@ extern "C" int64_t mk_paged_attention_workspace(const MkPagedCache *cache, const
     Batch bt;
     if (!cache || !batch) return refuse(MK_ERR_BAD_ARGUMENT, who, "null argument"), -1;
     int sms = 0;
-    if (read_cache(*cache, *batch, pool, bt, who) || sm_count(sms)) return -1;
+    if (read_cache(*cache, *batch, MK_PAGED_ATTENTION_MAX_SEQS, pool, bt, who) || sm_count(sms)) return -1;
     if (num_q_heads < 1 || num_q_heads % pool.kv_heads) return refuse(MK_ERR_UNSUPPORTED, who, "query heads are not a multiple of the KV heads"), -1;
     const long long bytes = attention_workspace(bt, pool, num_q_heads, sms);
     if (bytes < 0) refuse(MK_ERR_UNSUPPORTED, who, "more rows times positions than one call takes");
@@ -116,7 +116,7 @@ extern "C" int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch 
     if (!cache || !batch || !a) return refuse(MK_ERR_BAD_ARGUMENT, who, "null argument");
     AttentionParams p = {};
     Pool pool;
-    int code = read_cache(*cache, *batch, pool, p.bt, who);
+    int code = read_cache(*cache, *batch, MK_PAGED_ATTENTION_MAX_SEQS, pool, p.bt, who);
     if (code) return code;
     if (bad_rows(a->q, a->q_token_stride, a->q_head_stride) || !a->out || misaligned(a->out))
         return refuse(MK_ERR_BAD_ARGUMENT, who, "query or output rows null or not on 16-byte boundaries");

@@ -65,12 +65,6 @@ struct Tile {
     static constexpr int kMmaTiles = kTokens / 16;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -84,11 +78,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-// four E4M3 codes -> two f16 pairs (low codes first)
-__device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(lo), "=r"(hi) : "r"(codes));
-}
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (F16)
@@ -98,20 +87,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_b16(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int slot, int head, int page, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
-}
-
 // Row blocks of this launch: NT tiles of 8 query rows.
 template <int D, bool FP8, int NT>
 __global__ void __launch_bounds__(kWarps * 32)
@@ -709,18 +684,18 @@ static int row_tiles(const Batch &bt, int group, int max_count) {
     return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 
-bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens) {
+bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens, bool swizzle) {
     EncodeTiledFn fn = encode_tiled();
     if (!fn) return false;
     const int bytes = pool.fp8 ? 1 : 2;
-    const int panel = pool.head_dim * bytes < 128 ? pool.head_dim * bytes : 128;
+    const int panel = !swizzle || pool.head_dim * bytes < 128 ? pool.head_dim * bytes : 128;
     const cuuint64_t dims[4] = {(cuuint64_t)pool.head_dim, (cuuint64_t)pool.page_size, (cuuint64_t)pool.kv_heads, (cuuint64_t)pool.num_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)(pool.slot_stride * bytes), (cuuint64_t)(pool.head_stride * bytes),
                                    (cuuint64_t)(pool.page_stride * bytes)};
     const cuuint32_t box[4] = {(cuuint32_t)(panel / bytes), (cuuint32_t)box_tokens, 1, 1};
     const cuuint32_t elem[4] = {1, 1, 1, 1};
     return fn(map, pool.fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides,
-              box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, panel == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : panel == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -729,7 +704,7 @@ static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, 
     using T = Tile<D, FP8>;
     CUtensorMap map_k, map_v;
     const int box = pool.page_size < T::kTokens ? pool.page_size : T::kTokens;
-    if (!make_pool_map(&map_k, pool, pool.k, box) || !make_pool_map(&map_v, pool, pool.v, box)) {
+    if (!make_pool_map(&map_k, pool, pool.k, box, true) || !make_pool_map(&map_v, pool, pool.v, box, true)) {
         set_last_error("mk_paged_attention: cuTensorMapEncodeTiled refused the cache (driver without tensor-map support?)");
         return MK_ERR_UNSUPPORTED;
     }
@@ -773,19 +748,52 @@ int launch_decode(const AttentionParams &p, const Pool &pool, int sms, cudaStrea
     return pool.fp8 ? launch_decode_d<128, true>(p, pool, sms, st) : launch_decode_d<128, false>(p, pool, sms, st);
 }
 
-static int max_count_of_decode() { return 0x7fffffff; }
+// Most new tokens of a sequence that the few-row kernel takes: those whose rows fit one row block of
+// 32, so that it reads the cache once.  More rows are work for the tensor cores' large tiles.
+static int most_few(int group) { return group >= 32 ? 1 : 32 / group; }
+
+struct Plan {
+    bool few;             // the few-row kernel has (or may have) sequences
+    DecodeGrid decode;
+    PrefillGrid prefill;
+    long long ints, decode_floats, bytes;
+};
+
+static Plan plan_attention(const Batch &bt, const Pool &pool, int hq, int sms) {
+    Plan plan = {};
+    const int limit = most_few(hq / pool.kv_heads);
+    plan.few = bt.cu || bt.per_seq <= limit;
+    if (plan.few) plan.decode = decode_grid(pool, bt, hq, limit, sms);
+    plan.prefill = prefill_grid(pool, bt, hq, limit + 1, sms);
+    plan.ints = (bt.seqs + 1 + 3) & ~3;
+    plan.decode_floats = (plan.decode.partial_floats + 3) & ~3ll;
+    if (plan.decode.partial_floats || plan.prefill.partial_floats)
+        plan.bytes = 4 * (2 * plan.ints + plan.decode_floats + plan.prefill.partial_floats);
+    return plan;
+}
 
 long long attention_workspace(const Batch &bt, const Pool &pool, int hq, int sms) {
-    const DecodeGrid g = decode_grid(pool, bt, hq, max_count_of_decode(), sms);
-    if (g.too_many) return -1;
-    return g.split ? 4ll * (((bt.seqs + 1 + 3) & ~3) + g.partial_floats) : 0;
+    const Plan plan = plan_attention(bt, pool, hq, sms);
+    return plan.decode.too_many || plan.prefill.too_many ? -1 : plan.bytes;
 }
 
 int launch_attention(AttentionParams p, const Pool &pool, void *workspace, int sms, cudaStream_t st) {
-    p.max_count = max_count_of_decode();
-    p.prefix_out = reinterpret_cast<int *>(workspace);
-    p.partial = reinterpret_cast<float *>(workspace) + ((p.bt.seqs + 1 + 3) & ~3);
-    return launch_decode(p, pool, sms, st);
+    const Plan plan = plan_attention(p.bt, pool, p.hq, sms);
+    const int limit = most_few(p.group);
+    int code = 0;
+    float *floats = reinterpret_cast<float *>(workspace);
+    if (plan.few) {
+        p.max_count = limit;
+        p.prefix_out = plan.decode.split ? reinterpret_cast<int *>(workspace) : nullptr;
+        p.partial = floats + 2 * plan.ints;
+        code = launch_decode(p, pool, sms, st);
+    }
+    if (code == 0 && plan.prefill.ctas) {
+        p.prefix_out = plan.prefill.whole ? nullptr : reinterpret_cast<int *>(workspace) + plan.ints;
+        p.partial = floats + 2 * plan.ints + plan.decode_floats;
+        code = launch_prefill(p, pool, plan.prefill, limit + 1, st);
+    }
+    return code;
 }
 
 }  // namespace paged

@@ -1,5 +1,7 @@
-// What the kernels of attention over a paged cache share on the host.
+// What the kernels of attention over a paged cache share.
 #pragma once
+
+#include <cuda_fp16.h>
 
 #include "paged.cuh"
 
@@ -8,6 +10,31 @@ namespace paged {
 
 constexpr int kWarps = 4;                          // warps per CTA of the few-row kernel
 constexpr long long kWaitCycles = 2000000000ll;    // limit of a wait, about a second
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// four E4M3 codes -> two f16 pairs (low codes first)
+__device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_b16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int slot, int head, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
+}
 
 struct DecodeGrid {
     int ctas;
@@ -18,7 +45,18 @@ struct DecodeGrid {
 
 DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count, int sms);
 int launch_decode(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st);
-bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens);
+// tensor map [pages, heads, slots, dim] of a pool; boxes of box_tokens slots and up to 128 bytes with the matching swizzle, or of
+// whole rows without one
+bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens, bool swizzle);
+
+struct PrefillGrid {
+    int ctas;                       // 0: no sequence of the call can have enough rows
+    bool whole;                     // a CTA per row block; otherwise equal ranges of units, joined afterwards
+    bool too_many;
+    long long partial_floats;
+};
+PrefillGrid prefill_grid(const Pool &pool, const Batch &bt, int hq, int min_count, int sms);
+int launch_prefill(const AttentionParams &p, const Pool &pool, const PrefillGrid &grid, int min_count, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace mk
