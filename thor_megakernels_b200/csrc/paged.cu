@@ -56,11 +56,18 @@ static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs
 
 static bool bad_rows(const void *p, int64_t token, int64_t head) { return !p || misaligned(p) || token % 8 || head % 8 || token < 0 || head < 0; }
 
+// SMs of the current device, asked for once per device.
 static int sm_count(int &sms) {
+    static int known[64] = {};
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && device < 64 && known[device]) {
+        sms = known[device];
+        return 0;
+    }
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) set_last_error(cudaGetErrorString(e));
+    else if (device < 64) known[device] = sms;
     return (int)e;
 }
 

@@ -599,18 +599,20 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     }
 }
 
-// Joins the parts of the segments that several CTAs shared: one CTA per (sequence, KV head), its
-// warps taking every eighth part, four columns per lane.  Weights 2^(m_part - max m), parts in order.
+// Joins the parts of the segments that several CTAs shared: one CTA per (sequence, KV head).  A warp
+// takes a row, or with fewer than eight rows a share of a row's parts; its lanes read the statistics of
+// 32 parts at once, then the parts one after the other, D / 32 columns each.  The order of the sums is fixed.
 template <int D>
 __global__ void __launch_bounds__(256)
 join_kernel(const AttentionParams p, int rows_per_block, int unit, int grid) {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr int kCols = D / 32;
     const Batch &bt = p.bt;
     __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
     const int b = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int u_seq = __ldg(p.prefix_out + b), units = __ldg(p.prefix_out + bt.seqs);
-    if (__ldg(p.prefix_out + b + 1) == u_seq) return;
+    const int u_seq = __ldg(p.prefix_out + b), u_next = __ldg(p.prefix_out + b + 1), units = __ldg(p.prefix_out + bt.seqs);
+    if (u_next == u_seq) return;
     const int ctas = working_ctas(grid, units);
     int first, count;
     rows_of(bt, b, first, count);
@@ -620,53 +622,73 @@ join_kernel(const AttentionParams p, int rows_per_block, int unit, int grid) {
         const int tiles = max(block_tiles(length, count, p.group, rows_per_block, rb, unit), 1);
         const int u0 = at + head * tiles, u1 = u0 + tiles;
         at += tiles * p.hkv;
-        const int c0 = owner(u0, ctas, units), c1 = owner(u1 - 1, ctas, units);
-        if (c0 == c1) continue;   // written by its only CTA
+        const int c0 = owner(u0, ctas, units), c1 = owner(u1 - 1, ctas, units), parts = c1 - c0 + 1;
+        if (parts == 1) continue;   // written by its only CTA
         const int rows = min(rows_per_block, count * p.group - rb * rows_per_block);
-        for (int r = 0; r < rows; ++r) {
-            float M = -INFINITY, L = 0.f;
-            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto part_of = [&](int c) {
-                return p.partial + (((long long)c * 2 + (c == c0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
+        const int per = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps per row
+        for (int row0 = 0; row0 < rows; row0 += 8 / per) {
+            const int r = row0 + warp / per, sub = warp % per;
+            float M = -INFINITY, L = 0.f, O[kCols];
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) O[k] = 0.f;
+            auto part_of = [&](int i) {   // part i of the segment, this row
+                return p.partial + (((long long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
             };
-            for (int c = c0 + warp; c <= c1; c += 8) {
-                const float2 ml = *reinterpret_cast<const float2 *>(part_of(c) + D);
-                M = fmaxf(M, ml.x);
-            }
-            const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-            for (int c = c0 + warp; c <= c1; c += 8) {
-                const float *src = part_of(c);
-                const float2 ml = *reinterpret_cast<const float2 *>(src + D);
-                const float f = exp2_fast(ml.x - base);
-                L = fmaf(ml.y, f, L);
-                if (4 * lane < D) {
-                    const float2 x = *reinterpret_cast<const float2 *>(src + 4 * lane), y = *reinterpret_cast<const float2 *>(src + 4 * lane + 2);
-                    O.x = fmaf(x.x, f, O.x); O.y = fmaf(x.y, f, O.y); O.z = fmaf(y.x, f, O.z); O.w = fmaf(y.y, f, O.w);
+            if (r < rows) {
+                for (int base = sub; base < parts; base += 32 * per) {
+                    const int mine = base + lane * per;
+                    const float2 ml = mine < parts ? *reinterpret_cast<const float2 *>(part_of(mine) + D) : make_float2(-INFINITY, 0.f);
+                    float top = ml.x;
+#pragma unroll
+                    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                    top = fmaxf(top, M);
+                    const float zero = top == -INFINITY ? 0.f : top, corr = exp2_fast(M - zero), f = exp2_fast(ml.x - zero);
+                    float total = ml.y * f;
+#pragma unroll
+                    for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                    L = fmaf(L, corr, total);
+                    M = top;
+#pragma unroll
+                    for (int k = 0; k < kCols; ++k) O[k] *= corr;
+                    const int n = min(32, (parts - base + per - 1) / per);
+#pragma unroll 8
+                    for (int i = 0; i < n; ++i) {
+                        const float w = __shfl_sync(0xffffffffu, f, i);
+                        const float *src = part_of(base + i * per) + kCols * lane;
+#pragma unroll
+                        for (int k = 0; k < kCols; k += 2) {
+                            const float2 v = *reinterpret_cast<const float2 *>(src + k);
+                            O[k] = fmaf(v.x, w, O[k]);
+                            O[k + 1] = fmaf(v.y, w, O[k + 1]);
+                        }
+                    }
                 }
             }
-            __syncthreads();
-            if (lane == 0) {
-                sum_m[warp] = M;
-                sum_l[warp] = L;
-            }
-            if (4 * lane < D) *reinterpret_cast<float4 *>(&sum_o[warp][4 * lane]) = O;
-            __syncthreads();
-            if ((int)threadIdx.x < D) {
-                float top = -INFINITY;
+            if (per > 1) {   // the row's warps meet
+                __syncthreads();
+                if (lane == 0) { sum_m[warp] = M; sum_l[warp] = L; }
 #pragma unroll
-                for (int w = 0; w < 8; ++w) top = fmaxf(top, sum_m[w]);
-                top = top == -INFINITY ? 0.f : top;
-                float total = 0.f, value = 0.f;
+                for (int k = 0; k < kCols; ++k) sum_o[warp][kCols * lane + k] = O[k];
+                __syncthreads();
+                M = -INFINITY;
+                for (int w = 0; w < per; ++w) M = fmaxf(M, sum_m[warp - sub + w]);
+                const float zero = M == -INFINITY ? 0.f : M;
+                L = 0.f;
 #pragma unroll
-                for (int w = 0; w < 8; ++w) {
-                    const float f = exp2_fast(sum_m[w] - top);
-                    total = fmaf(sum_l[w], f, total);
-                    value = fmaf(sum_o[w][threadIdx.x], f, value);
+                for (int k = 0; k < kCols; ++k) O[k] = 0.f;
+                for (int w = 0; w < per; ++w) {
+                    const float f = exp2_fast(sum_m[warp - sub + w] - zero);
+                    L = fmaf(sum_l[warp - sub + w], f, L);
+#pragma unroll
+                    for (int k = 0; k < kCols; ++k) O[k] = fmaf(sum_o[warp - sub + w][kCols * lane + k], f, O[k]);
                 }
+            }
+            if (r < rows && sub == 0) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
                 const int pair = rb * rows_per_block + r;
-                p.out[((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + threadIdx.x] =
-                    __float2bfloat16_rn(total == 0.f ? 0.f : value / total);
+                bf16 *dst = p.out + ((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + kCols * lane;
+#pragma unroll
+                for (int k = 0; k < kCols; k += 2) *reinterpret_cast<__nv_bfloat162 *>(dst + k) = __floats2bfloat162_rn(O[k] * inv, O[k + 1] * inv);
             }
         }
     }
@@ -709,7 +731,8 @@ static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, 
         return MK_ERR_UNSUPPORTED;
     }
     const size_t smem = 1024 + kWarps * T::kRing + (size_t)(p.bt.seqs + 1) * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<D, FP8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static bool allowed[64] = {};
+    cudaError_t e = allow_smem((const void *)decode_kernel<D, FP8, NT>, allowed);
     if (e != cudaSuccess) return (int)e;
     const DecodeGrid grid = decode_grid(pool, p.bt, p.hq, p.max_count, sms);
     e = launch_pdl(decode_kernel<D, FP8, NT>, dim3(grid.ctas), dim3(kWarps * 32), smem, st, map_k, map_v, p);

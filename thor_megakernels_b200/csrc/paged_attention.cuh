@@ -36,6 +36,20 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
                  ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
 }
 
+// Lets `kernel` use as much shared memory as a device has (once per device and kernel: `done` is the kernel's own).
+inline cudaError_t allow_smem(const void *kernel, bool (&done)[64]) {
+    int device = 0, most = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && done[device])) return e;
+    e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes);
+    if (e == cudaSuccess && device < 64) done[device] = true;
+    return e;
+}
+
 struct DecodeGrid {
     int ctas;
     bool split;                     // a segment may be shared by several CTAs

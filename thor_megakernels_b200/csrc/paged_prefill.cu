@@ -841,7 +841,8 @@ static int launch_prefill_t(const PrefillParams &pp, const Pool &pool, const Pre
         return MK_ERR_UNSUPPORTED;
     }
     const size_t smem = 1024 + sizeof(typename T::Smem) + (size_t)(pp.a.bt.seqs + 1) * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static bool allowed[64] = {};
+    cudaError_t e = allow_smem((const void *)prefill_kernel<D, FP8>, allowed);
     if (e == cudaSuccess) e = launch_pdl(prefill_kernel<D, FP8>, dim3(grid.ctas), dim3(T::kThreads), smem, st, map_k, map_v, pp);
     if (e == cudaSuccess && !grid.whole)
         e = launch_pdl(join_blocks_kernel<D>, dim3(pp.a.bt.seqs, pp.a.hkv, D / kJoinColumns), dim3(kBlockRows), 0, st, pp, grid.ctas);
