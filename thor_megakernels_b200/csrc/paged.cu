@@ -140,7 +140,7 @@ extern "C" int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch 
     p.q = (const bf16 *)a->q; p.q_token = a->q_token_stride; p.q_head = a->q_head_stride;
     p.out = (bf16 *)a->out;
     p.k_scales = pool.k_scales; p.v_scales = pool.v_scales;
-    p.hq = a->num_q_heads; p.hkv = pool.kv_heads; p.group = a->num_q_heads / pool.kv_heads;
+    p.hq = a->num_q_heads; p.hkv = pool.kv_heads; p.group = fast_div(a->num_q_heads / pool.kv_heads);
     p.scale_log2e = a->scale * 1.4426950408889634f;
     code = launch_attention(p, pool, a->workspace, sms, (cudaStream_t)stream);
     if (code > 0 && code < 10000) set_last_error(cudaGetErrorString((cudaError_t)code));

@@ -148,8 +148,7 @@ __device__ __forceinline__ int sequence_of_row(const Batch &bt, int t) {
 template <int D, int ITERS, bool FP8, bool LIN>
 __global__ void __launch_bounds__(kAppendThreads)
 append_kernel(const AppendParams p) {
-    pdl_launch_dependents();
-    pdl_wait();
+    pdl_wait();   // and no early start for the next kernel: see paged.cuh
     constexpr int kChunks = D / 8;                         // threads per row
     constexpr int kHalf = kAppendThreads / 2;
     constexpr int kRows = kHalf / kChunks;                 // rows per pass of half a CTA

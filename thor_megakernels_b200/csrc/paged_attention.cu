@@ -38,6 +38,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 #include <stdio.h>
 
@@ -52,6 +53,9 @@ void set_last_error(const char *msg);  // megakernel.cu
 
 namespace paged {
 
+// CTAs per SM, by what their registers allow
+__host__ __device__ constexpr int resident_ctas(int row_tiles) { return row_tiles == 1 ? 3 : 2; }
+
 template <int D, bool FP8>
 struct Tile {
     static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
@@ -59,10 +63,22 @@ struct Tile {
     static constexpr int kPanels = kRowBytes / kPanelBytes;
     static constexpr int kTokens = kRowBytes == 256 ? 16 : 32;              // positions per warp tile
     static constexpr int kBytes = kTokens * kRowBytes;                      // keys (and values)
-    static constexpr int kStages = kRowBytes == 64 ? 6 : 3;                 // 24 KiB per warp
+    static constexpr int kStages = kRowBytes == 64 ? 4 : 2;                 // 16 KiB per warp
     static constexpr int kRing = kStages * 2 * kBytes;
     static constexpr int kUnit = kWarps * kTokens;                          // positions per unit
     static constexpr int kMmaTiles = kTokens / 16;
+};
+
+constexpr int kSegmentCost = 1;   // of a segment besides its tiles, in units
+
+template <int D, bool FP8, int NT>
+struct __align__(1024) DecodeSmem {
+    uint8_t ring[kWarps][Tile<D, FP8>::kRing];
+    float merge[2][8 * NT * D];
+    float stat_m[kWarps][8 * NT], stat_l[kWarps][8 * NT];
+    uint64_t full[kWarps][Tile<D, FP8>::kStages];
+    int scan[kWarps];
+    int prefix[1];   // [seqs + 1]
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -87,168 +103,118 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Row blocks of this launch: NT tiles of 8 query rows.
+// NT: tiles of 8 query rows per row block.
 template <int D, bool FP8, int NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, resident_ctas(NT))
 decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
     using T = Tile<D, FP8>;
-    constexpr int kRowsPerBlock = 8 * NT;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t full[kWarps][T::kStages];
-    __shared__ float stat_m[kWarps][kRowsPerBlock], stat_l[kWarps][kRowsPerBlock];
-    __shared__ int scan_s[kWarps];
-    int *prefix = reinterpret_cast<int *>(smem + kWarps * T::kRing);   // [seqs + 1]
+    using Smem = DecodeSmem<D, FP8, NT>;
+    constexpr int kRows = 8 * NT;
+    constexpr Cut kCut = {kRows, T::kUnit, kSegmentCost};
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const Batch &bt = p.bt;
     pdl_launch_dependents();
     if (lane == 0)
-        for (int i = 0; i < T::kStages; ++i) mbar_init(&full[warp][i], 1);
+        for (int i = 0; i < T::kStages; ++i) mbar_init(&sm.full[warp][i], 1);
     fence_barrier_init();
     pdl_wait();
+    Walk walk;
+    plan_walk<kWarps * 32>(bt, p.hkv, p.group, kCut, 0, p.max_count, sm.prefix, sm.scan, walk);
 
-    // units of the sequences before each one
-    {
-        const int per = (bt.seqs + kWarps * 32 - 1) / (kWarps * 32);
-        const int b0 = min((int)threadIdx.x * per, bt.seqs), b1 = min(b0 + per, bt.seqs);
-        int sum = 0;
-        for (int b = b0; b < b1; ++b) {
-            int first, count;
-            rows_of(bt, b, first, count);
-            const int units = count > p.max_count ? 0 : sequence_units(length_of(bt, b), count, p.group, kRowsPerBlock, T::kUnit, p.hkv);
-            prefix[b + 1] = units;
-            sum += units;
-        }
-        int incl = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += v;
-        }
-        if (lane == 31) scan_s[warp] = incl;
-        __syncthreads();
-        int before = incl - sum;
-        for (int w = 0; w < warp; ++w) before += scan_s[w];
-        for (int b = b0; b < b1; ++b) {
-            before += prefix[b + 1];
-            prefix[b + 1] = before;
-        }
-        if (threadIdx.x == 0) prefix[0] = 0;
-        __syncthreads();
-    }
-    const int units = prefix[bt.seqs];
-    if (blockIdx.x == 0 && p.prefix_out)
-        for (int b = threadIdx.x; b <= bt.seqs; b += kWarps * 32) p.prefix_out[b] = prefix[b];
-    const int ctas = working_ctas(gridDim.x, units);
-    if ((int)blockIdx.x >= ctas) return;
-    int u = first_unit(blockIdx.x, ctas, units);
-    const int u_end = first_unit(blockIdx.x + 1, ctas, units);
-
-    uint8_t *ring = smem + warp * T::kRing;
-    const uint32_t ring_s = smem_addr(ring);
-    uint32_t stage = 0, parity = 0;
+    const uint32_t ring = smem_addr(sm.ring[warp]);
     const int page_mask = (1 << bt.page_shift) - 1;
-    constexpr int kPagesPerTile = 2;   // at most: 32 positions over pages of 16
+    const bool two = page_mask + 1 < T::kTokens;   // a tile of 32 positions over two pages of 16
+    constexpr int kPages = 2;
 
-    int b = 0;
-    while (u < u_end) {
-        // the segment that unit u lies in: sequence, row block, head, tile range
-        {
-            int lo = b, hi = bt.seqs - 1;   // last sequence with prefix <= u
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (prefix[mid] <= u) lo = mid;
-                else hi = mid - 1;
-            }
-            b = lo;
-        }
-        int first, count;
-        rows_of(bt, b, first, count);
-        const int length = length_of(bt, b);
-        int rest = u - prefix[b], rb = 0, tiles;
-        while (true) {
-            tiles = max(block_tiles(length, count, p.group, kRowsPerBlock, rb, T::kUnit), 1);
-            if (rest < tiles * p.hkv) break;
-            rest -= tiles * p.hkv;
-            ++rb;
-        }
-        const int head = rest / tiles, tile0 = rest % tiles;
-        const int tile1 = min(tiles, tile0 + (u_end - u));
-        const bool whole = tile0 == 0 && tile1 == tiles;
-        const int rows = min(kRowsPerBlock, count * p.group - rb * kRowsPerBlock);
-        const int last_token = min(((rb + 1) * kRowsPerBlock - 1) / p.group, count - 1);
-        const int seen = visible(length, count, last_token);                        // positions this block looks at
-        const int all_see = visible(length, count, rb * kRowsPerBlock / p.group);   // positions that every row sees
-        const int end = min(tile1 * T::kUnit, seen);
-        // this warp's tiles: positions from + i * kUnit
-        const int from = tile0 * T::kUnit + warp * T::kTokens;
-        const int n = end > from ? (end - from + T::kUnit - 1) / T::kUnit : 0;
-
-        // pages (and scales) of 32 tiles at a time, one tile per lane
-        const int *table = bt.table + b * bt.table_stride;
-        int page_cur[kPagesPerTile], page_next[kPagesPerTile];
-        float ks_cur[kPagesPerTile], vs_cur[kPagesPerTile], ks_next[kPagesPerTile], vs_next[kPagesPerTile];
-        auto load_pages = [&](int i0, int (&page)[kPagesPerTile]) {
+    // this warp's tiles of a segment: positions from + i * kUnit, i < n
+    struct Share {
+        int from, n, seen;      // seen: positions the row block looks at
+        const int *table;
+    };
+    auto share_of = [&](const Segment &s) {
+        Share h;
+        h.seen = min(s.tile1 * T::kUnit, visible(s.length, s.count, min(div((s.rb + 1) * kRows - 1, p.group), s.count - 1)));
+        h.from = s.tile0 * T::kUnit + warp * T::kTokens;
+        h.n = h.seen > h.from ? (h.seen - h.from + T::kUnit - 1) / T::kUnit : 0;
+        h.table = bt.table + s.b * bt.table_stride;
+        return h;
+    };
+    // pages of 32 tiles from i0 on, one tile per lane
+    auto load_pages = [&](const Share &h, int i0, int (&page)[kPages]) {
 #pragma unroll
-            for (int h = 0; h < kPagesPerTile; ++h) {
-                const int pos = from + (i0 + lane) * T::kUnit + h * 16;
-                page[h] = -1;
-                if (i0 + lane < n && pos < end && (h * 16) < T::kTokens) {
-                    const int id = __ldg(table + (pos >> bt.page_shift));
-                    if (id >= bt.num_pages) atomicOr(bt.error, kErrorIndex);
-                    else page[h] = id;
-                }
-            }
-        };
-        auto load_scales = [&](const int (&page)[kPagesPerTile], float (&ks)[kPagesPerTile], float (&vs)[kPagesPerTile]) {
-            if constexpr (FP8) {
-#pragma unroll
-                for (int h = 0; h < kPagesPerTile; ++h) {
-                    ks[h] = 1.f;
-                    vs[h] = 0.f;
-                    if (page[h] >= 0) {
-                        const long long at = (long long)page[h] * p.hkv + head;
-                        ks[h] = __ldg(p.k_scales + at);
-                        vs[h] = log2f(fmaxf(__ldg(p.v_scales + at), 0x1p-100f));
-                    }
-                }
-            }
-        };
-        load_pages(0, page_cur);
-#pragma unroll
-        for (int h = 0; h < kPagesPerTile; ++h) page_next[h] = -1;
-
-        // fill of tile i into ring stage `st`
-        auto issue = [&](int i, uint32_t st, int cur0) {
-            int page[kPagesPerTile];
-            const bool next = i >= cur0 + 32;
-#pragma unroll
-            for (int h = 0; h < kPagesPerTile; ++h) page[h] = __shfl_sync(0xffffffffu, next ? page_next[h] : page_cur[h], i & 31);
-            if (lane == 0) {
-                const int pos = from + i * T::kUnit;
-                const uint32_t dst = ring_s + st * 2 * T::kBytes;
-                mbar_arrive_expect_tx(&full[warp][st], 2 * T::kBytes);
-                const int boxes = page_mask + 1 < T::kTokens ? T::kTokens / 16 : 1;   // pages of 16 come in two boxes
-                for (int h = 0; h < boxes; ++h) {
-#pragma unroll
-                    for (int panel = 0; panel < T::kPanels; ++panel) {
-                        const uint32_t at = dst + panel * T::kTokens * T::kPanelBytes + h * 16 * T::kPanelBytes;
-                        const int x = panel * T::kPanelBytes / (FP8 ? 1 : 2), slot = (pos + h * 16) & page_mask;
-                        tma_load_4d(at, &map_k, x, slot, head, page[h], &full[warp][st]);
-                        tma_load_4d(at + T::kBytes, &map_v, x, slot, head, page[h], &full[warp][st]);
-                    }
-                }
-            }
-        };
-        {
-            uint32_t st = stage;
-            for (int i = 0; i < min(n, T::kStages); ++i) {
-                issue(i, st, 0);
-                if (++st == T::kStages) st = 0;
+        for (int k = 0; k < kPages; ++k) {
+            const int pos = h.from + (i0 + lane) * T::kUnit + 16 * k;
+            page[k] = -1;
+            if (i0 + lane < h.n && pos < h.seen && (k == 0 || two)) {
+                const int id = __ldg(h.table + (pos >> bt.page_shift));
+                if (id >= bt.num_pages) atomicOr(bt.error, kErrorIndex);
+                else page[k] = id;
             }
         }
-        load_scales(page_cur, ks_cur, vs_cur);
+    };
+    auto load_scales = [&](const int (&page)[kPages], int head, float (&ks)[kPages], float (&vs)[kPages]) {
+        if constexpr (FP8) {
+#pragma unroll
+            for (int k = 0; k < kPages; ++k) {
+                ks[k] = 1.f;
+                vs[k] = 0.f;
+                if (page[k] >= 0) {
+                    const long long at = (long long)page[k] * p.hkv + head;
+                    ks[k] = __ldg(p.k_scales + at);
+                    vs[k] = log2f(fmaxf(__ldg(p.v_scales + at), 0x1p-100f));
+                }
+            }
+        }
+    };
+    // copy of a tile into ring stage st
+    auto issue = [&](const Share &h, int head, int i, const int (&pages)[kPages], uint32_t st) {
+        const int page0 = __shfl_sync(0xffffffffu, pages[0], i & 31), page1 = two ? __shfl_sync(0xffffffffu, pages[1], i & 31) : 0;
+        if (lane == 0) {
+            const int pos = h.from + i * T::kUnit;
+            const uint32_t dst = ring + st * 2 * T::kBytes;
+            uint64_t *bar = &sm.full[warp][st];
+            mbar_arrive_expect_tx(bar, 2 * T::kBytes);
+#pragma unroll
+            for (int panel = 0; panel < T::kPanels; ++panel) {
+                const uint32_t at = dst + panel * T::kTokens * T::kPanelBytes;
+                const int x = panel * T::kPanelBytes / (FP8 ? 1 : 2);
+                tma_load_4d(at, &map_k, x, pos & page_mask, head, page0, bar);
+                tma_load_4d(at + T::kBytes, &map_v, x, pos & page_mask, head, page0, bar);
+                if (two) {
+                    tma_load_4d(at + 16 * T::kPanelBytes, &map_k, x, 0, head, page1, bar);
+                    tma_load_4d(at + 16 * T::kPanelBytes + T::kBytes, &map_v, x, 0, head, page1, bar);
+                }
+            }
+        }
+    };
+
+    uint32_t stage = 0, parity = 0;   // the tile consumed next
+    uint32_t fill = 0;                // the stage filled next
+    int in_flight = 0, odd = 0;       // filled stages; segments so far, mod 2
+    JoinEntry entry = {0, 0, 0, 0};
+    Segment cur, next;
+    Share mine, mine_next;
+    int page_cur[kPages], page_next[kPages];   // of 32 tiles; page_next: the 32 after them, in this segment or the next
+    float ks_cur[kPages], vs_cur[kPages], ks_next[kPages], vs_next[kPages];
+    int ahead = 0;                             // tiles of the next segment that have been asked for
+    bool have = next_segment(bt, p.hkv, p.group, kCut, walk, cur);
+    if (have) {
+        mine = share_of(cur);
+        load_pages(mine, 0, page_cur);
+    }
+
+    while (have) {
+        int asked = ahead;   // tiles of this segment that have been asked for
+        ahead = 0;
+        while (in_flight < T::kStages && asked < mine.n && asked < 32) {
+            issue(mine, cur.head, asked++, page_cur, fill);
+            if (++fill == T::kStages) fill = 0;
+            ++in_flight;
+        }
+        load_scales(page_cur, cur.head, ks_cur, vs_cur);
 
         // query fragments: row g of tile nt, with the columns' order of the key fragments
         uint32_t qf[D / 16][NT][2];
@@ -256,10 +222,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         int limit[NT][2];       // positions those rows see
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g, pair = rb * kRowsPerBlock + r;
-            const bool real = r < rows;
-            const bf16 *qp = p.q + (long long)(first + (real ? pair / p.group : 0)) * p.q_token +
-                             (long long)(head * p.group + (real ? pair % p.group : 0)) * p.q_head;
+            const int r = nt * 8 + g, pair = cur.rb * kRows + r;
+            const bool real = r < cur.rows;
+            const bf16 *qp = p.q + (long long)(cur.first + (real ? div(pair, p.group) : 0)) * p.q_token +
+                             (long long)(cur.head * p.group.d + (real ? pair - div(pair, p.group) * p.group.d : 0)) * p.q_head;
             float unscale = 1.f;
             if constexpr (FP8) {
                 uint32_t raw[D / 16][2];
@@ -269,13 +235,15 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     const uint2 v = real ? __ldg(reinterpret_cast<const uint2 *>(qp + 16 * ks + 4 * t)) : make_uint2(0u, 0u);
                     raw[ks][0] = v.x;
                     raw[ks][1] = v.y;
+                }
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float a = fabsf(bf16_lo(raw[ks][i])), c = fabsf(bf16_hi(raw[ks][i]));
                         if (a < INFINITY) amax = fmaxf(amax, a);
                         if (c < INFINITY) amax = fmaxf(amax, c);
                     }
-                }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 // 2^e with amax / 2^e in [2^14, 2^15); e stays where both it and its inverse are normal numbers
@@ -295,11 +263,17 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                q_scale[nt][e] = p.scale_log2e * __shfl_sync(0xffffffffu, unscale, (2 * t + e) * 4);
+                q_scale[nt][e] = FP8 ? p.scale_log2e * __shfl_sync(0xffffffffu, unscale, (2 * t + e) * 4) : p.scale_log2e;
                 const int r2 = nt * 8 + 2 * t + e;
-                limit[nt][e] = r2 < rows ? visible(length, count, (rb * kRowsPerBlock + r2) / p.group) : 0;
+                limit[nt][e] = r2 < cur.rows ? visible(cur.length, cur.count, div(cur.rb * kRows + r2, p.group)) : 0;
             }
         }
+        const int all_see = visible(cur.length, cur.count, div(cur.rb * kRows, p.group));   // positions that every row sees
+
+        // the next segment, while the first copies of this one are under way
+        const bool have_next = next_segment(bt, p.hkv, p.group, kCut, walk, next);
+        if (have_next) mine_next = share_of(next);
+        else mine_next.n = 0;
 
         float m[NT][2], l[NT][2];
         float o[D / 16][NT][4];
@@ -310,47 +284,45 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) o[c][nt][0] = o[c][nt][1] = o[c][nt][2] = o[c][nt][3] = 0.f;
         }
+        bool next_paged = false;   // page_next holds the next segment's first pages
 
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < mine.n; ++i) {
             const int cur0 = i & ~31;
-            if ((i & 31) == 0 && i) {
+            const bool last = cur0 + 32 >= mine.n;
+            if (i == cur0) {
+                if (i) {
 #pragma unroll
-                for (int h = 0; h < kPagesPerTile; ++h) { page_cur[h] = page_next[h]; ks_cur[h] = ks_next[h]; vs_cur[h] = vs_next[h]; }
+                    for (int k = 0; k < kPages; ++k) { page_cur[k] = page_next[k]; ks_cur[k] = ks_next[k]; vs_cur[k] = vs_next[k]; }
+                }
+                if (!last) load_pages(mine, cur0 + 32, page_next);
+                else if (have_next) load_pages(mine_next, 0, page_next);
+                next_paged = last && have_next;
             }
-            if ((i & 31) == 12) load_pages(cur0 + 32, page_next);        // well before the first use, ...
-            if ((i & 31) == 24) load_scales(page_next, ks_next, vs_next);
-            // this tile's scales
+            if ((i & 31) == 24 && !last) load_scales(page_next, cur.head, ks_next, vs_next);
+
             float ks[T::kMmaTiles], vs[T::kMmaTiles];
-            bool absent = false;   // a position range without a page
-            const bool two = page_mask + 1 < T::kTokens;
+            const int pg0 = __shfl_sync(0xffffffffu, page_cur[0], i & 31), pg1 = two ? __shfl_sync(0xffffffffu, page_cur[1], i & 31) : pg0;
 #pragma unroll
             for (int mt = 0; mt < T::kMmaTiles; ++mt) {
-                const int h = two ? mt : 0;
-                if constexpr (FP8) {
-                    const float k0 = __shfl_sync(0xffffffffu, ks_cur[0], i & 31), k1 = __shfl_sync(0xffffffffu, ks_cur[1], i & 31);
-                    const float v0 = __shfl_sync(0xffffffffu, vs_cur[0], i & 31), v1 = __shfl_sync(0xffffffffu, vs_cur[1], i & 31);
-                    ks[mt] = h ? k1 : k0;
-                    vs[mt] = h ? v1 : v0;
+                if (FP8 && (mt == 0 || two)) {
+                    ks[mt] = __shfl_sync(0xffffffffu, ks_cur[mt], i & 31);
+                    vs[mt] = __shfl_sync(0xffffffffu, vs_cur[mt], i & 31);
                 } else {
-                    ks[mt] = 1.f;
-                    vs[mt] = 0.f;
+                    ks[mt] = FP8 ? ks[0] : 1.f;
+                    vs[mt] = FP8 ? vs[0] : 0.f;
                 }
             }
-            const int pg0 = __shfl_sync(0xffffffffu, page_cur[0], i & 31), pg1 = __shfl_sync(0xffffffffu, page_cur[1], i & 31);
-            absent = pg0 < 0 || (two && T::kMmaTiles > 1 && pg1 < 0);
 
-            const uint32_t kt = ring_s + stage * 2 * T::kBytes, vt = kt + T::kBytes;
-            const int pos0 = from + i * T::kUnit;
-            {
-                bool ok = mbar_try_wait(&full[warp][stage], parity);
-                if (!ok) {
-                    const long long began = clock64();
-                    while (!(ok = mbar_try_wait(&full[warp][stage], parity)))
-                        if (clock64() - began > kWaitCycles) break;
-                    if (!ok && lane == 0) atomicOr(bt.error, kErrorWait);
-                }
-                __syncwarp();
+            const uint32_t kt = ring + stage * 2 * T::kBytes, vt = kt + T::kBytes;
+            const int pos0 = mine.from + i * T::kUnit;
+            if (!mbar_try_wait(&sm.full[warp][stage], parity)) {
+                const long long began = clock64();
+                bool ok;
+                while (!(ok = mbar_try_wait(&sm.full[warp][stage], parity)))
+                    if (clock64() - began > kWaitCycles) break;
+                if (!ok && lane == 0) atomicOr(bt.error, kErrorWait);
             }
+            __syncwarp();
 
             // scores [position][query row]
             float sc[T::kMmaTiles][NT][4];
@@ -390,26 +362,26 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             }
 
             // rows that look past their own last position, positions past the sequence, pages that are not there
-            const bool masked = absent || pos0 + T::kTokens > all_see;
+            const bool masked = pg0 < 0 || pg1 < 0 || pos0 + T::kTokens > all_see;
             if (masked) {
                 // A value that is not finite must not meet the zero weight of a row that does not see it: take it out
                 // of the tile, and give it to the rows that see it by hand.
-                uint32_t odd = 0;
+                uint32_t bad = 0;
                 for (int c = lane; c < T::kTokens * (T::kRowBytes / 16); c += 32) {
                     const int r = c / (T::kRowBytes / 16), pos = pos0 + r;
                     const uint32_t addr = chunk_at(vt, r, c % (T::kRowBytes / 16));
-                    if (pos >= length) {
+                    if (pos >= cur.length) {
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
                     } else if (pos >= all_see) {
                         uint32_t w[4];
                         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) odd |= FP8 ? __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu) : __vcmpeq2(w[j] & 0x7f807f80u, 0x7f807f80u);
+                        for (int j = 0; j < 4; ++j) bad |= FP8 ? not_finite_e4m3(w[j]) : not_finite_b16(w[j]);
                     }
                 }
                 __syncwarp();
-                if (__any_sync(0xffffffffu, odd != 0)) {
-                    for (int r = max(all_see - pos0, 0); r < min(T::kTokens, length - pos0); ++r) {
+                if (__any_sync(0xffffffffu, bad != 0)) {
+                    for (int r = max(all_see - pos0, 0); r < min(T::kTokens, cur.length - pos0); ++r) {
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
@@ -419,8 +391,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                                 uint32_t bits;
                                 if constexpr (FP8) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bits) : "r"(at));
                                 else asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bits) : "r"(at));
-                                const bool bad = FP8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u;
-                                if (bad) {
+                                if (FP8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u) {
                                     const float value = FP8 ? __int_as_float(0x7fffffff) : __uint_as_float(bits << 16);
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt)
@@ -433,7 +404,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     __syncwarp();
                     for (int c = lane; c < T::kTokens * (T::kRowBytes / 4); c += 32) {
                         const int r = c / (T::kRowBytes / 4), byte = c % (T::kRowBytes / 4) * 4;
-                        if (pos0 + r < all_see || pos0 + r >= length) continue;
+                        if (pos0 + r < all_see || pos0 + r >= cur.length) continue;
                         const uint32_t at = chunk_at(vt, r, byte / 16) + byte % 16;
                         uint32_t w;
                         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
@@ -448,7 +419,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             // online softmax of rows 2t, 2t + 1 of every tile over this tile's positions
             uint32_t pf[T::kMmaTiles][NT][2], pf_lo[T::kMmaTiles][NT][2];
             bool rescale = false;
-            float corr[NT][2];
+            float corr[NT][2], inv_vs[T::kMmaTiles];
+#pragma unroll
+            for (int mt = 0; mt < T::kMmaTiles; ++mt) inv_vs[mt] = FP8 ? exp2_fast(-vs[mt]) : 1.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -462,8 +435,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                             float x = FP8 ? fmaf(sc[mt][nt][2 * h + e], c, vs[mt]) : sc[mt][nt][2 * h + e] * c;
                             if (masked) {
                                 const int pos = pos0 + mt * 16 + h * 8 + g;
-                                const bool there = (two && mt == 1 ? pg1 : pg0) >= 0;
-                                if (!(there && pos < limit[nt][e])) x = -INFINITY;
+                                if (!((mt == 1 ? pg1 : pg0) >= 0 && pos < limit[nt][e])) x = -INFINITY;
                             }
                             sc[mt][nt][2 * h + e] = x;
                             mx = fmaxf(mx, x);
@@ -482,8 +454,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                         const float w0 = exp2_fast(sc[mt][nt][e] - base), w1 = exp2_fast(sc[mt][nt][2 + e] - base);
                         sc[mt][nt][e] = w0;
                         sc[mt][nt][2 + e] = w1;
-                        if constexpr (FP8) add = fmaf(w0 + w1, exp2_fast(-vs[mt]), add);
-                        else add += w0 + w1;
+                        add = fmaf(w0 + w1, inv_vs[mt], add);
                     }
                     l[nt][e] = fmaf(l[nt][e], corr[nt][e], add);
                 }
@@ -538,158 +509,218 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                 }
             }
             __syncwarp();
-            if (i + T::kStages < n) issue(i + T::kStages, stage, cur0);
+            --in_flight;
             if (++stage == T::kStages) { stage = 0; parity ^= 1u; }
+            // ask for what comes next: this segment's tiles, then the next one's
+            while (in_flight < T::kStages) {
+                if (asked < mine.n) {
+                    if (asked < cur0 + 32) issue(mine, cur.head, asked, page_cur, fill);
+                    else issue(mine, cur.head, asked, page_next, fill);
+                    ++asked;
+                } else if (next_paged && ahead < mine_next.n && ahead < 32) {
+                    issue(mine_next, next.head, ahead, page_next, fill);
+                    ++ahead;
+                } else {
+                    break;
+                }
+                if (++fill == T::kStages) fill = 0;
+                ++in_flight;
+            }
         }
 
-        // the warps' states meet in shared memory (each warp's ring is idle now)
-        float *mine = reinterpret_cast<float *>(ring);   // [row][D]
+        // The warps' states meet, in an order that does not depend on timing: two warps leave theirs in shared memory, the
+        // others add them, and one adds the last pair and writes.  The roles swap from segment to segment, so that a
+        // buffer's next writer is the warp that read it last.
+        const int swapped = odd, role = swapped ? 3 - warp : warp;
+        odd ^= 1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int off = 4; off < 32; off *= 2) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
-                const int r = nt * 8 + 2 * t + e;
                 if (g == 0) {
-                    stat_m[warp][r] = m[nt][e];
-                    stat_l[warp][r] = l[nt][e];
+                    sm.stat_m[warp][nt * 8 + 2 * t + e] = m[nt][e];
+                    sm.stat_l[warp][nt * 8 + 2 * t + e] = l[nt][e];
                 }
+            }
+        auto leave = [&](float *buffer) {   // lane-major: one fragment register of all lanes side by side
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c)
+                    *reinterpret_cast<float4 *>(buffer + ((nt * (D / 16) + c) * 32 + lane) * 4) = make_float4(o[c][nt][0], o[c][nt][1], o[c][nt][2], o[c][nt][3]);
+        };
+        auto add = [&](const float *buffer, const float (&f)[NT][2]) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const float4 v = *reinterpret_cast<const float4 *>(buffer + ((nt * (D / 16) + c) * 32 + lane) * 4);
+                    o[c][nt][0] = fmaf(v.x, f[nt][0], o[c][nt][0]);
+                    o[c][nt][1] = fmaf(v.y, f[nt][1], o[c][nt][1]);
+                    o[c][nt][2] = fmaf(v.z, f[nt][0], o[c][nt][2]);
+                    o[c][nt][3] = fmaf(v.w, f[nt][1], o[c][nt][3]);
+                }
+        };
+        if (role >= 2) leave(sm.merge[role - 2]);
+        __syncthreads();
+        float M[NT][2], L[NT][2];
+        if (role < 2) {
+            const int partner = swapped ? 1 - role : 2 + role;   // the warp whose state lies in merge[role]
+            float f_own[NT][2], f_partner[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = nt * 8 + 2 * t + e;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.stat_m[w][r]);
+                    const float base = top == -INFINITY ? 0.f : top;
+                    float total = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) total = fmaf(sm.stat_l[w][r], exp2_fast(sm.stat_m[w][r] - base), total);
+                    M[nt][e] = top;
+                    L[nt][e] = total;
+                    f_own[nt][e] = exp2_fast(m[nt][e] - base);
+                    f_partner[nt][e] = exp2_fast(sm.stat_m[partner][r] - base);
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int d = FP8 ? 16 * c + 2 * g + half : 16 * c + 8 * half + g;
-                        mine[r * D + d] = o[c][nt][2 * half + e];
-                    }
-            }
+                    for (int j = 0; j < 4; ++j) o[c][nt][j] *= f_own[nt][j & 1];
+            add(sm.merge[role], f_partner);
+            if (role == 1) leave(sm.merge[1]);
         }
         __syncthreads();
-        // slot of the workspace: 0 continues a segment that an earlier CTA began, 1 begins one that a later CTA ends
-        float *part = p.partial + ((long long)blockIdx.x * 2 + (tile0 == 0 ? 1 : 0)) * kRowsPerBlock * (D + 2);
-        for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kWarps * 32) {
-            const int r = idx / (D / 4), d = idx % (D / 4) * 4;
-            float M = -INFINITY;
+        if (role == 0) {
+            float ones[NT][2];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, stat_m[w][r]);
-            const float base = M == -INFINITY ? 0.f : M;
-            float L = 0.f;
-            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int nt = 0; nt < NT; ++nt) ones[nt][0] = ones[nt][1] = 1.f;
+            add(sm.merge[1], ones);
+            const bool complete = cur.begins && cur.ends;
+            float *part = p.partial + ((long long)blockIdx.x * 2 + (cur.begins ? 1 : 0)) * kRows * (D + 2);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float f = exp2_fast(stat_m[w][r] - base);
-                L = fmaf(stat_l[w][r], f, L);
-                const float4 v = *reinterpret_cast<const float4 *>(smem + w * T::kRing + (r * D + d) * 4);
-                O.x = fmaf(v.x, f, O.x); O.y = fmaf(v.y, f, O.y); O.z = fmaf(v.z, f, O.z); O.w = fmaf(v.w, f, O.w);
-            }
-            if (whole) {
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                const int pair = rb * kRowsPerBlock + r;
-                bf16 *dst = p.out + ((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + d;
-                bo::store_bf16x4(dst, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
-            } else {
-                *reinterpret_cast<float2 *>(part + r * (D + 2) + d) = make_float2(O.x, O.y);
-                *reinterpret_cast<float2 *>(part + r * (D + 2) + d + 2) = make_float2(O.z, O.w);
-                if (d == 0) *reinterpret_cast<float2 *>(part + r * (D + 2) + D) = make_float2(M, L);
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring's plain writes, before the next copies into it
-        __syncthreads();
-        u += tile1 - tile0;
-    }
-}
-
-// Joins the parts of the segments that several CTAs shared: one CTA per (sequence, KV head).  A warp
-// takes a row, or with fewer than eight rows a share of a row's parts; its lanes read the statistics of
-// 32 parts at once, then the parts one after the other, D / 32 columns each.  The order of the sums is fixed.
-template <int D>
-__global__ void __launch_bounds__(256)
-join_kernel(const AttentionParams p, int rows_per_block, int unit, int grid) {
-    pdl_launch_dependents();
-    pdl_wait();
-    constexpr int kCols = D / 32;
-    const Batch &bt = p.bt;
-    __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
-    const int b = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int u_seq = __ldg(p.prefix_out + b), u_next = __ldg(p.prefix_out + b + 1), units = __ldg(p.prefix_out + bt.seqs);
-    if (u_next == u_seq) return;
-    const int ctas = working_ctas(grid, units);
-    int first, count;
-    rows_of(bt, b, first, count);
-    const int length = length_of(bt, b), blocks = block_count(count, p.group, rows_per_block);
-    int at = u_seq;
-    for (int rb = 0; rb < blocks; ++rb) {
-        const int tiles = max(block_tiles(length, count, p.group, rows_per_block, rb, unit), 1);
-        const int u0 = at + head * tiles, u1 = u0 + tiles;
-        at += tiles * p.hkv;
-        const int c0 = owner(u0, ctas, units), c1 = owner(u1 - 1, ctas, units), parts = c1 - c0 + 1;
-        if (parts == 1) continue;   // written by its only CTA
-        const int rows = min(rows_per_block, count * p.group - rb * rows_per_block);
-        const int per = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps per row
-        for (int row0 = 0; row0 < rows; row0 += 8 / per) {
-            const int r = row0 + warp / per, sub = warp % per;
-            float M = -INFINITY, L = 0.f, O[kCols];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) O[k] = 0.f;
-            auto part_of = [&](int i) {   // part i of the segment, this row
-                return p.partial + (((long long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
-            };
-            if (r < rows) {
-                for (int base = sub; base < parts; base += 32 * per) {
-                    const int mine = base + lane * per;
-                    const float2 ml = mine < parts ? *reinterpret_cast<const float2 *>(part_of(mine) + D) : make_float2(-INFINITY, 0.f);
-                    float top = ml.x;
+                for (int e = 0; e < 2; ++e) {
+                    const int r = nt * 8 + 2 * t + e;
+                    if (r >= cur.rows) continue;
+                    const int pair = cur.rb * kRows + r;
+                    bf16 *dst = p.out + ((long long)(cur.first + div(pair, p.group)) * p.hq + cur.head * p.group.d + pair - div(pair, p.group) * p.group.d) * D;
+                    const float inv = L[nt][e] == 0.f ? 0.f : 1.f / L[nt][e];
 #pragma unroll
-                    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                    top = fmaxf(top, M);
-                    const float zero = top == -INFINITY ? 0.f : top, corr = exp2_fast(M - zero), f = exp2_fast(ml.x - zero);
-                    float total = ml.y * f;
-#pragma unroll
-                    for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-                    L = fmaf(L, corr, total);
-                    M = top;
-#pragma unroll
-                    for (int k = 0; k < kCols; ++k) O[k] *= corr;
-                    const int n = min(32, (parts - base + per - 1) / per);
-#pragma unroll 8
-                    for (int i = 0; i < n; ++i) {
-                        const float w = __shfl_sync(0xffffffffu, f, i);
-                        const float *src = part_of(base + i * per) + kCols * lane;
-#pragma unroll
-                        for (int k = 0; k < kCols; k += 2) {
-                            const float2 v = *reinterpret_cast<const float2 *>(src + k);
-                            O[k] = fmaf(v.x, w, O[k]);
-                            O[k + 1] = fmaf(v.y, w, O[k + 1]);
+                    for (int c = 0; c < D / 16; ++c) {
+                        const float x = o[c][nt][e], y = o[c][nt][2 + e];
+                        if constexpr (FP8) {   // columns 16 c + 2 g and the next one
+                            if (complete) *reinterpret_cast<__nv_bfloat162 *>(dst + 16 * c + 2 * g) = __floats2bfloat162_rn(x * inv, y * inv);
+                            else *reinterpret_cast<float2 *>(part + r * (D + 2) + 16 * c + 2 * g) = make_float2(x, y);
+                        } else {               // columns 16 c + g and 16 c + 8 + g
+                            if (complete) {
+                                dst[16 * c + g] = __float2bfloat16_rn(x * inv);
+                                dst[16 * c + 8 + g] = __float2bfloat16_rn(y * inv);
+                            } else {
+                                part[r * (D + 2) + 16 * c + g] = x;
+                                part[r * (D + 2) + 16 * c + 8 + g] = y;
+                            }
                         }
                     }
+                    if (!complete && g == 0) *reinterpret_cast<float2 *>(part + r * (D + 2) + D) = make_float2(M[nt][e], L[nt][e]);
+                }
+        }
+        if (cur.parts > 1) entry = JoinEntry{cur.parts, cur.first, cur.rb * kRows, (cur.head << 16) | cur.rows};
+        if (have_next && !next_paged) load_pages(mine_next, 0, page_next);   // this warp had no tile in the segment
+        have = have_next;
+        cur = next;
+        mine = mine_next;
+#pragma unroll
+        for (int k = 0; k < kPages; ++k) page_cur[k] = page_next[k];
+    }
+    if (p.entries && threadIdx.x == 0) p.entries[blockIdx.x] = entry;
+}
+
+// Joins the parts of the segments that several CTAs shared: one CTA for the segment that begins in CTA
+// blockIdx.x's range, if there is one, and for a share of its rows.  A warp takes a row, or with fewer than
+// eight rows a share of a row's parts; its lanes read the statistics of 32 parts at once, then the parts one
+// after the other, D / 32 columns each.  The order of the sums is fixed.
+template <int D>
+__global__ void __launch_bounds__(256)
+join_kernel(const AttentionParams p, int rows_per_block) {
+    pdl_wait();   // and no early start for the next kernel: see paged.cuh
+    constexpr int kCols = D / 32;
+    __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
+    const int4 raw = __ldg(reinterpret_cast<const int4 *>(p.entries + blockIdx.x));
+    const JoinEntry e = {raw.x, raw.y, raw.z, raw.w};
+    if (e.parts == 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = e.head_rows & 0xffff, head = e.head_rows >> 16;
+    const int share = (rows + gridDim.y - 1) / gridDim.y, row_end = min(rows, (int)(blockIdx.y + 1) * share);   // rows of this CTA
+    const int per = share > 4 ? 1 : share > 2 ? 2 : share > 1 ? 4 : 8;                                          // warps per row
+    for (int row0 = blockIdx.y * share; row0 < row_end; row0 += 8 / per) {
+        const int r = row0 + warp / per, sub = warp % per;
+        float M = -INFINITY, L = 0.f, O[kCols];
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) O[k] = 0.f;
+        auto part_of = [&](int i) {   // part i of the segment, this row
+            return p.partial + (((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
+        };
+        if (r < row_end) {
+            for (int base = sub; base < e.parts; base += 32 * per) {
+                const int mine = base + lane * per;
+                const float2 ml = mine < e.parts ? *reinterpret_cast<const float2 *>(part_of(mine) + D) : make_float2(-INFINITY, 0.f);
+                float top = ml.x;
+#pragma unroll
+                for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                top = fmaxf(top, M);
+                const float zero = top == -INFINITY ? 0.f : top, corr = exp2_fast(M - zero), f = exp2_fast(ml.x - zero);
+                float total = ml.y * f;
+#pragma unroll
+                for (int off = 16; off; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                L = fmaf(L, corr, total);
+                M = top;
+#pragma unroll
+                for (int k = 0; k < kCols; ++k) O[k] *= corr;
+                const int n = min(32, (e.parts - base + per - 1) / per);
+#pragma unroll 8
+                for (int i = 0; i < n; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, f, i);
+                    const float *src = part_of(base + i * per) + kCols * lane;
+#pragma unroll
+                    for (int k = 0; k < kCols; k += 2) {
+                        const float2 v = *reinterpret_cast<const float2 *>(src + k);
+                        O[k] = fmaf(v.x, w, O[k]);
+                        O[k + 1] = fmaf(v.y, w, O[k + 1]);
+                    }
                 }
             }
-            if (per > 1) {   // the row's warps meet
-                __syncthreads();
-                if (lane == 0) { sum_m[warp] = M; sum_l[warp] = L; }
+        }
+        if (per > 1) {   // the row's warps meet
+            __syncthreads();
+            if (lane == 0) { sum_m[warp] = M; sum_l[warp] = L; }
 #pragma unroll
-                for (int k = 0; k < kCols; ++k) sum_o[warp][kCols * lane + k] = O[k];
-                __syncthreads();
-                M = -INFINITY;
-                for (int w = 0; w < per; ++w) M = fmaxf(M, sum_m[warp - sub + w]);
-                const float zero = M == -INFINITY ? 0.f : M;
-                L = 0.f;
+            for (int k = 0; k < kCols; ++k) sum_o[warp][kCols * lane + k] = O[k];
+            __syncthreads();
+            M = -INFINITY;
+            for (int w = 0; w < per; ++w) M = fmaxf(M, sum_m[warp - sub + w]);
+            const float zero = M == -INFINITY ? 0.f : M;
+            L = 0.f;
 #pragma unroll
-                for (int k = 0; k < kCols; ++k) O[k] = 0.f;
-                for (int w = 0; w < per; ++w) {
-                    const float f = exp2_fast(sum_m[warp - sub + w] - zero);
-                    L = fmaf(sum_l[warp - sub + w], f, L);
+            for (int k = 0; k < kCols; ++k) O[k] = 0.f;
+            for (int w = 0; w < per; ++w) {
+                const float f = exp2_fast(sum_m[warp - sub + w] - zero);
+                L = fmaf(sum_l[warp - sub + w], f, L);
 #pragma unroll
-                    for (int k = 0; k < kCols; ++k) O[k] = fmaf(sum_o[warp - sub + w][kCols * lane + k], f, O[k]);
-                }
+                for (int k = 0; k < kCols; ++k) O[k] = fmaf(sum_o[warp - sub + w][kCols * lane + k], f, O[k]);
             }
-            if (r < rows && sub == 0) {
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                const int pair = rb * rows_per_block + r;
-                bf16 *dst = p.out + ((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + kCols * lane;
+        }
+        if (r < row_end && sub == 0) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            const int pair = e.pair + r;
+            bf16 *dst = p.out + ((long long)(e.row + div(pair, p.group)) * p.hq + head * p.group.d + pair - div(pair, p.group) * p.group.d) * D + kCols * lane;
 #pragma unroll
-                for (int k = 0; k < kCols; k += 2) *reinterpret_cast<__nv_bfloat162 *>(dst + k) = __floats2bfloat162_rn(O[k] * inv, O[k + 1] * inv);
-            }
+            for (int k = 0; k < kCols; k += 2) *reinterpret_cast<__nv_bfloat162 *>(dst + k) = __floats2bfloat162_rn(O[k] * inv, O[k + 1] * inv);
         }
     }
 }
@@ -724,26 +755,26 @@ bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box
 template <int D, bool FP8, int NT>
 static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
     using T = Tile<D, FP8>;
+    using DecodeSmemOf = DecodeSmem<D, FP8, NT>;
     CUtensorMap map_k, map_v;
     const int box = pool.page_size < T::kTokens ? pool.page_size : T::kTokens;
     if (!make_pool_map(&map_k, pool, pool.k, box, true) || !make_pool_map(&map_v, pool, pool.v, box, true)) {
         set_last_error("mk_paged_attention: cuTensorMapEncodeTiled refused the cache (driver without tensor-map support?)");
         return MK_ERR_UNSUPPORTED;
     }
-    const size_t smem = 1024 + kWarps * T::kRing + (size_t)(p.bt.seqs + 1) * sizeof(int);
+    const size_t smem = offsetof(DecodeSmemOf, prefix) + (size_t)(p.bt.seqs + 1) * sizeof(int);
     static bool allowed[64] = {};
     cudaError_t e = allow_smem((const void *)decode_kernel<D, FP8, NT>, allowed);
     if (e != cudaSuccess) return (int)e;
     const DecodeGrid grid = decode_grid(pool, p.bt, p.hq, p.max_count, sms);
     e = launch_pdl(decode_kernel<D, FP8, NT>, dim3(grid.ctas), dim3(kWarps * 32), smem, st, map_k, map_v, p);
-    if (e == cudaSuccess && grid.split)
-        e = launch_pdl(join_kernel<D>, dim3(p.bt.seqs, p.hkv), dim3(256), 0, st, p, 8 * NT, T::kUnit, grid.ctas);
+    if (e == cudaSuccess && grid.split) e = launch_pdl(join_kernel<D>, dim3(grid.ctas, grid.join_turns), dim3(256), 0, st, p, 8 * NT);
     return (int)e;
 }
 
 template <int D, bool FP8>
 static int launch_decode_d(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
-    switch (row_tiles(p.bt, p.group, p.max_count)) {
+    switch (row_tiles(p.bt, p.group.d, p.max_count)) {
     case 1: return launch_decode_t<D, FP8, 1>(p, pool, sms, st);
     case 2: return launch_decode_t<D, FP8, 2>(p, pool, sms, st);
     default: return launch_decode_t<D, FP8, 4>(p, pool, sms, st);
@@ -756,9 +787,13 @@ DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count,
     const int group = hq / pool.kv_heads, rows = 8 * row_tiles(bt, group, max_count);
     const long long tiles = (((long long)bt.max_pages << bt.page_shift) + unit - 1) / unit;
     const long long blocks = bt.cu ? (long long)bt.tokens * group / rows + bt.seqs : (long long)bt.seqs * block_count(bt.per_seq, group, rows);
-    const long long most = blocks * pool.kv_heads * (tiles > 0 ? tiles : 1);
+    const long long most = blocks * pool.kv_heads * (tiles + kSegmentCost);
     DecodeGrid g;
-    g.ctas = (int)(most < 2ll * sms ? most : 2ll * sms);   // two resident CTAs per SM
+    const long long resident = (long long)resident_ctas(rows / 8) * sms;
+    g.ctas = (int)(most < resident ? most : resident);
+    // segments to join: as many as there are row blocks, or CTAs where that is less; rows are dealt out until the GPU is full
+    const long long joins = blocks * pool.kv_heads < g.ctas ? blocks * pool.kv_heads : g.ctas, turns = (sms + joins - 1) / joins;
+    g.join_turns = (int)(turns < rows ? turns : rows);
     g.split = tiles > 1;
     g.too_many = most > 0x7fffffffll;
     g.partial_floats = g.split ? (long long)g.ctas * 2 * rows * (pool.head_dim + 2) : 0;
@@ -779,7 +814,7 @@ struct Plan {
     bool few;             // the few-row kernel has (or may have) sequences
     DecodeGrid decode;
     PrefillGrid prefill;
-    long long ints, decode_floats, bytes;
+    long long entries, decode_floats, bytes;   // entries: of both kernels, in words
 };
 
 static Plan plan_attention(const Batch &bt, const Pool &pool, int hq, int sms) {
@@ -788,10 +823,10 @@ static Plan plan_attention(const Batch &bt, const Pool &pool, int hq, int sms) {
     plan.few = bt.cu || bt.per_seq <= limit;
     if (plan.few) plan.decode = decode_grid(pool, bt, hq, limit, sms);
     plan.prefill = prefill_grid(pool, bt, hq, limit + 1, sms);
-    plan.ints = (bt.seqs + 1 + 3) & ~3;
+    plan.entries = 4ll * ((plan.decode.split ? plan.decode.ctas : 0) + plan.prefill.ctas);
     plan.decode_floats = (plan.decode.partial_floats + 3) & ~3ll;
     if (plan.decode.partial_floats || plan.prefill.partial_floats)
-        plan.bytes = 4 * (2 * plan.ints + plan.decode_floats + plan.prefill.partial_floats);
+        plan.bytes = 4 * (plan.entries + plan.decode_floats + plan.prefill.partial_floats);
     return plan;
 }
 
@@ -802,18 +837,18 @@ long long attention_workspace(const Batch &bt, const Pool &pool, int hq, int sms
 
 int launch_attention(AttentionParams p, const Pool &pool, void *workspace, int sms, cudaStream_t st) {
     const Plan plan = plan_attention(p.bt, pool, p.hq, sms);
-    const int limit = most_few(p.group);
+    const int limit = most_few(p.group.d);
     int code = 0;
     float *floats = reinterpret_cast<float *>(workspace);
     if (plan.few) {
         p.max_count = limit;
-        p.prefix_out = plan.decode.split ? reinterpret_cast<int *>(workspace) : nullptr;
-        p.partial = floats + 2 * plan.ints;
+        p.entries = plan.decode.split ? reinterpret_cast<JoinEntry *>(workspace) : nullptr;
+        p.partial = floats + plan.entries;
         code = launch_decode(p, pool, sms, st);
     }
     if (code == 0 && plan.prefill.ctas) {
-        p.prefix_out = plan.prefill.whole ? nullptr : reinterpret_cast<int *>(workspace) + plan.ints;
-        p.partial = floats + 2 * plan.ints + plan.decode_floats;
+        p.entries = reinterpret_cast<JoinEntry *>(workspace) + (plan.decode.split ? plan.decode.ctas : 0);
+        p.partial = floats + plan.entries + plan.decode_floats;
         code = launch_prefill(p, pool, plan.prefill, limit + 1, st);
     }
     return code;

@@ -22,6 +22,9 @@ __device__ __forceinline__ void codes_to_f16(uint32_t codes, uint32_t &lo, uint3
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(lo), "=r"(hi) : "r"(codes));
 }
+// non-zero where one of the codes / values of a word is not finite: all ones in the exponent (and, E4M3, the mantissa) carry
+__device__ __forceinline__ uint32_t not_finite_e4m3(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t not_finite_b16(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -36,24 +39,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
                  ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
 }
 
-// Lets `kernel` use as much shared memory as a device has (once per device and kernel: `done` is the kernel's own).
-inline cudaError_t allow_smem(const void *kernel, bool (&done)[64]) {
-    int device = 0, most = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess || (device < 64 && done[device])) return e;
-    e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
-    if (e != cudaSuccess) return e;
-    cudaFuncAttributes attr;
-    e = cudaFuncGetAttributes(&attr, kernel);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes);
-    if (e == cudaSuccess && device < 64) done[device] = true;
-    return e;
-}
-
 struct DecodeGrid {
     int ctas;
     bool split;                     // a segment may be shared by several CTAs
     bool too_many;                  // more units than 32 bits count
+    int join_turns;                 // CTAs that share a segment's rows in the join
     long long partial_floats;
 };
 
@@ -65,7 +55,6 @@ bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box
 
 struct PrefillGrid {
     int ctas;                       // 0: no sequence of the call can have enough rows
-    bool whole;                     // a CTA per row block; otherwise equal ranges of units, joined afterwards
     bool too_many;
     long long partial_floats;
 };

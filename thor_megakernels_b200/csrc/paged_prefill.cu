@@ -11,13 +11,14 @@
 // What bounds it: per 128 x 128 tile the tensor core needs 4 x 128 x 128 x D flops - 1024 clocks
 // at D = 128 - and the softmax 128 x 128 exponentials - 1024 clocks of the special function unit.
 // Two row tiles alternate, so that one's softmax runs under the other's products:
-//     S0(j+1) follows O0(j), S1(j+1) follows O1(j) in the issue order,
-// and weights take S's place in tensor memory.  The output is rescaled only when the running
+// S(j+1) follows O(j) in each row tile's order of issue, and weights take S's place in tensor memory, in
+// halves: the first half's product runs under the second half's exponentials.  The output is rescaled only when the running
 // maximum has grown by more than 2^8 since the last time (weights stay below 256, sums are fp32);
 // after the first tiles that is rare.
 //
 // Warp roles: 0-3 and 4-7 softmax of row tile 0 and 1 (and query loading, epilogue), 8 loader (TMA,
-// one box per page), 9 tensor-memory allocation and MMA issue, and for the 8-bit cache 10 and 11
+// one box per page), 9 and 10 MMA issue for one row tile each (9 also allocates tensor memory), 11 planner
+// (finds the CTA's segments ahead of the others), and for the 8-bit cache 12-15
 // converters: E4M3 codes land as they are in a small ring and become f16 (exact) in the swizzled
 // operand tiles; queries are f16 scaled by a power of two per row, page scales enter at the scores
 // and the value scale joins the exponent, as in paged_attention.cu.  A bf16 cache goes from TMA
@@ -26,14 +27,15 @@
 // Values that are not finite and lie at positions some rows do not see (or behind the end) are
 // taken out of the tile by the warp that fills it; rows that do see them get them in the epilogue.
 //
-// Work split.  With at least two row blocks per SM every CTA takes one, those with the longest
-// cache first; otherwise units (row block, tile) are dealt out in equal consecutive ranges and a
-// second kernel joins the parts.
+// Work split.  One CTA per SM takes an equal consecutive range of units (tiles, and two for what a row
+// block costs besides); the next row block's queries and tiles are fetched during the last one's epilogue.
+// Row blocks that a range's end cuts are joined by a second kernel.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 #include <stdio.h>
 
@@ -53,11 +55,32 @@ constexpr int kBlockRows = 256;
 constexpr int kPanelBytes = 128 * 128;     // 128 rows of one 128-byte swizzle row
 constexpr int kChunks = kTileTokens / 16;  // a page is at least 16 positions
 constexpr int kBadBuffers = 4;
+// 2^f, |f| <= 1/2: minimax in relative error (2.6e-6), found with the Remez exchange
+__device__ constexpr float kExp2[5] = {0.9999992847f, 0.6931217909f, 0.2402474433f, 0.0559178591f, 0.0095701022f};
+constexpr int kPolynomialOf8 = 2;          // of eight neighbouring exponentials, so many (pairs) are computed that way
+constexpr float kLeastFactor = 1.17549435e-38f;   // of a score: minus infinity (a masked score) times it stays what it is
+
+// What the roles need of a segment besides its place.
+struct Shape {
+    int n[2];           // tiles of the two row tiles in it
+    int most;           // the larger of them: tiles that are loaded
+    int all_see;        // positions that every row sees
+};
+// One segment as the planner hands it to the other roles.
+struct Order {
+    Segment seg;
+    Shape shape;
+    int valid;          // 0: there are no more
+};
+constexpr int kOrders = 4;
 
 template <int D, bool FP8>
 struct Prefill {
-    static constexpr int kConverters = 64;
-    static constexpr int kThreads = FP8 ? 320 + kConverters : 320;
+    static constexpr int kConverters = 128;
+    static constexpr int kThreads = FP8 ? 512 : 384;
+    // Registers per thread: 128 (four warpgroups) or 168 (three) at launch; then a row of 128 scores stays in the softmax threads'.
+    static constexpr int kSoftmaxRegisters = 200, kOtherRegisters = FP8 ? 56 : 104;
+    static_assert(2 * kSoftmaxRegisters + (FP8 ? 2 : 1) * kOtherRegisters <= (FP8 ? 4 * 128 : 3 * 168), "within the launch's registers");
     static constexpr int kPanels = D / 64;
     static constexpr int kOperandBytes = kPanels * kPanelBytes;   // 128 rows x D two-byte elements
     static constexpr int kRawTokens = kTileTokens / 2, kRawStages = FP8 ? 3 : 1;
@@ -69,89 +92,42 @@ struct Prefill {
         uint8_t v[2][kOperandBytes];
         uint8_t raw[kRawStages][kRawBytes];
         uint64_t raw_full[kRawStages], raw_empty[kRawStages], k_full[2], k_empty[2], v_full[2], v_empty[2], v_raw;
-        uint64_t s_full[2], p_full[2], o_full[2], q_full, drain;
+        uint64_t order_full[kOrders], order_empty[kOrders];
+        Order order[kOrders];
+        uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drain[2];
         float ks[4][kChunks], ev[4][kChunks], iev[4][kChunks];   // by tile counter mod 4: key scale, log2 of the value scale and its inverse
-        int general[4];                                          // the tile needs them
-        int bad[kBadBuffers][kBadKinds][D];                              // first position whose value in a column is NaN, +inf, -inf
+        int bad[kBadBuffers][kBadKinds][D];                      // first position whose value in a column is NaN, +inf, -inf
         int bad_any[kBadBuffers];
         uint32_t tmem_base;
         int failed;
         int scan[kThreads / 32];
+        int prefix[1];                                           // [seqs + 1]
     };
 };
+
+constexpr int kPrefillCost = 2;            // of a segment besides its tiles, in tiles
+__device__ constexpr Cut kPrefillCut = {kBlockRows, kTileTokens, kPrefillCost};
 
 struct PrefillParams {
     AttentionParams a;
     int min_count;      // sequences with fewer new tokens are the other kernel's
-    int whole;          // every CTA takes one row block
 };
 
-struct Segment {
-    int b, first, count, length, rb, head, tile0, tile1, rows;
-    bool complete;      // the row block's tiles are all in this segment
-    int n[2];           // tiles of the two row tiles in it
-    int all_see;        // positions that every row sees
-};
-
-__device__ __forceinline__ void describe(const AttentionParams &p, Segment &s) {
-    s.rows = min(kBlockRows, s.count * p.group - s.rb * kBlockRows);
-    s.all_see = visible(s.length, s.count, s.rb * kBlockRows / p.group);
+__device__ __forceinline__ Shape shape_of(const AttentionParams &p, const Segment &s) {
+    Shape h;
+    h.all_see = visible(s.length, s.count, div(s.rb * kBlockRows, p.group));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int last = min(s.rows, 128 * (i + 1)) - 1;
-        int n = 0;
+        h.n[i] = 0;
         if (last >= 128 * i) {
-            const int seen = visible(s.length, s.count, (s.rb * kBlockRows + last) / p.group);
-            n = max(min((seen + kTileTokens - 1) / kTileTokens, s.tile1) - s.tile0, 0);
+            const int seen = visible(s.length, s.count, div(s.rb * kBlockRows + last, p.group));
+            h.n[i] = max(min((seen + kTileTokens - 1) / kTileTokens, s.tile1) - s.tile0, 0);
         }
-        s.n[i] = n;
     }
+    h.most = max(h.n[0], h.n[1]);
+    return h;
 }
-
-// Walks over a CTA's segments.  Every role runs its own copy.
-struct Walk {
-    const int *prefix;
-    int u, u_end, b;
-    bool done;
-    __device__ __forceinline__ bool next(const PrefillParams &p, Segment &s) {
-        if (u >= u_end) return false;
-        const AttentionParams &a = p.a;
-        int lo = b, hi = a.bt.seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (prefix[mid] <= u) lo = mid;
-            else hi = mid - 1;
-        }
-        b = s.b = lo;
-        rows_of(a.bt, b, s.first, s.count);
-        s.length = length_of(a.bt, b);
-        int rest = u - prefix[b];
-        if (p.whole) {
-            s.rb = block_count(s.count, a.group, kBlockRows) - 1 - rest / a.hkv;
-            s.head = rest % a.hkv;
-            s.tile0 = 0;
-            s.tile1 = max(block_tiles(s.length, s.count, a.group, kBlockRows, s.rb, kTileTokens), 1);
-            s.complete = true;
-            u += 1;
-        } else {
-            s.rb = 0;
-            int tiles;
-            while (true) {
-                tiles = max(block_tiles(s.length, s.count, a.group, kBlockRows, s.rb, kTileTokens), 1);
-                if (rest < tiles * a.hkv) break;
-                rest -= tiles * a.hkv;
-                ++s.rb;
-            }
-            s.head = rest / tiles;
-            s.tile0 = rest % tiles;
-            s.tile1 = min(tiles, s.tile0 + (u_end - u));
-            s.complete = s.tile0 == 0 && s.tile1 == tiles;
-            u += s.tile1 - s.tile0;
-        }
-        describe(a, s);
-        return true;
-    }
-};
 
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *failed) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -169,6 +145,29 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
     return true;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
+// 2^x of a pair on the fused multiply-add pipe: x = n + f with n the nearest integer, 2^f (|f| <= 1/2) by a degree-4
+// polynomial, times 2^n put together from n's bits (0 from n = -127 down, so that what is not seen weighs nothing).
+__device__ __forceinline__ uint64_t exp2_polynomial(uint64_t x) {
+    float x0, x1;
+    split_f32(x, x0, x1);
+    x = pair_f32(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+    const float magic = 12582912.f;   // 1.5 * 2^23: the sum's low bits are n
+    const uint64_t shifted = add_f32x2(x, pair_f32(magic, magic));
+    const uint64_t f = fma_f32x2(add_f32x2(shifted, pair_f32(-magic, -magic)), pair_f32(-1.f, -1.f), x);
+    uint64_t poly = pair_f32(kExp2[4], kExp2[4]);
+#pragma unroll
+    for (int k = 3; k >= 0; --k) poly = fma_f32x2(poly, f, pair_f32(kExp2[k], kExp2[k]));
+    float s0, s1;
+    split_f32(shifted, s0, s1);
+    return mul_f32x2(poly, pair_f32(__uint_as_float((__float_as_uint(s0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(s1) << 23) + 0x3f800000u)));
+}
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // byte offset of 16-byte chunk c of row r in an operand tile (panels of 64 elements, 128-byte swizzle)
@@ -179,9 +178,8 @@ __global__ void __launch_bounds__(Prefill<D, FP8>::kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefillParams pp) {
     using T = Prefill<D, FP8>;
     using Smem = typename T::Smem;
-    extern __shared__ uint8_t smem_raw[];
-    Smem &s = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    int *prefix = reinterpret_cast<int *>(&s + 1);   // [seqs + 1]
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem &s = *reinterpret_cast<Smem *>(smem_raw);
     const AttentionParams &p = pp.a;
     const Batch &bt = p.bt;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -191,72 +189,35 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.k_full[i], FP8 ? T::kConverters : 1);
             mbar_init(&s.v_full[i], FP8 ? T::kConverters : 1);
-            mbar_init(&s.k_empty[i], 1);
-            mbar_init(&s.v_empty[i], 1);
+            mbar_init(&s.k_empty[i], 2);   // one arrival per row tile
+            mbar_init(&s.v_empty[i], 2);
+            mbar_init(&s.q_full[i], 128);
             mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i], 128);
+            mbar_init(&s.p_full[i][0], 128);
+            mbar_init(&s.p_full[i][1], 128);
             mbar_init(&s.o_full[i], 1);
         }
         for (int i = 0; i < T::kRawStages; ++i) {
             mbar_init(&s.raw_full[i], 1);
             mbar_init(&s.raw_empty[i], T::kConverters);
         }
+        for (int i = 0; i < kOrders; ++i) {
+            mbar_init(&s.order_full[i], 1);
+            mbar_init(&s.order_empty[i], 8 + 1 + 2 + (FP8 ? T::kConverters / 32 : 0));   // softmax and converter warps, loader, MMA
+        }
         mbar_init(&s.v_raw, 1);
-        mbar_init(&s.q_full, 256);
-        mbar_init(&s.drain, 1);
+        mbar_init(&s.drain[0], 1);
+        mbar_init(&s.drain[1], 1);
         s.failed = 0;
         fence_barrier_init();
     }
     pdl_wait();
-
-    // units (or row blocks) of the sequences before each one
-    {
-        const int per = (bt.seqs + T::kThreads - 1) / T::kThreads;
-        const int b0 = min((int)threadIdx.x * per, bt.seqs), b1 = min(b0 + per, bt.seqs);
-        int sum = 0;
-        for (int b = b0; b < b1; ++b) {
-            int first, count;
-            rows_of(bt, b, first, count);
-            int units = 0;
-            if (count >= pp.min_count)
-                units = pp.whole ? block_count(count, p.group, kBlockRows) * p.hkv
-                                 : sequence_units(length_of(bt, b), count, p.group, kBlockRows, kTileTokens, p.hkv);
-            prefix[b + 1] = units;
-            sum += units;
-        }
-        int incl = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += v;
-        }
-        if (lane == 31) s.scan[warp] = incl;
-        __syncthreads();
-        int before = incl - sum;
-        for (int w = 0; w < warp; ++w) before += s.scan[w];
-        for (int b = b0; b < b1; ++b) {
-            before += prefix[b + 1];
-            prefix[b + 1] = before;
-        }
-        if (threadIdx.x == 0) prefix[0] = 0;
-        __syncthreads();
-    }
-    const int units = prefix[bt.seqs];
-    if (blockIdx.x == 0 && p.prefix_out && !pp.whole)
-        for (int b = threadIdx.x; b <= bt.seqs; b += T::kThreads) p.prefix_out[b] = prefix[b];
     Walk walk;
-    walk.prefix = prefix;
-    walk.b = 0;
-    if (pp.whole) {
-        walk.u = blockIdx.x;
-        walk.u_end = min((int)blockIdx.x + 1, units);
-    } else {
-        const int ctas = working_ctas(gridDim.x, units);
-        walk.u = (int)blockIdx.x < ctas ? first_unit(blockIdx.x, ctas, units) : 0;
-        walk.u_end = (int)blockIdx.x < ctas ? first_unit(blockIdx.x + 1, ctas, units) : 0;
+    plan_walk<T::kThreads>(bt, p.hkv, p.group, kPrefillCut, pp.min_count, 0x7fffffff, s.prefix, s.scan, walk);
+    if (walk.u >= walk.u_end) {   // the whole CTA
+        if (threadIdx.x == 0) p.entries[blockIdx.x] = JoinEntry{0, 0, 0, 0};
+        return;
     }
-    if (walk.u >= walk.u_end) return;   // the whole CTA
-
     // Tensor memory is taken only after the kernel before this one has ended, and the next kernel is let in
     // only after that: nobody who holds it waits for somebody who wants it.
     if (warp == 9) {
@@ -271,7 +232,27 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const int page_size = 1 << bt.page_shift;
 
     Segment seg;
+    Shape shape;
+    uint32_t orders = 0;   // taken so far
+    // The next segment from the planner; `arrives`: this thread gives the entry back for its warp.
+    auto advance = [&](bool arrives) {
+        const int at = orders & (kOrders - 1);
+        if (!wait_bar(&s.order_full[at], (orders / kOrders) & 1, failed)) return false;
+        seg = s.order[at].seg;
+        shape = s.order[at].shape;
+        const bool valid = s.order[at].valid != 0;
+        ++orders;
+        if (arrives) mbar_arrive(&s.order_empty[at]);
+        return valid;
+    };
+    auto advance_warp = [&]() {   // all lanes
+        const int at = orders & (kOrders - 1);
+        const bool valid = __all_sync(0xffffffffu, advance(false));
+        if (lane == 0) mbar_arrive(&s.order_empty[at]);
+        return valid;
+    };
     if (warp < 8) {
+        take_registers<T::kSoftmaxRegisters>();
         // ------------------------------------------------------------------ softmax of one row tile
         const int i = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -279,55 +260,58 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         uint32_t s_parity = 0, o_parity = 0;
         int tile_ctr = 0, bearing = 0;   // tiles and tile-bearing segments of this CTA so far
         bool ok = true;
-        while (ok && walk.next(pp, seg)) {
+        // Queries: a warp loads its 32 rows side by side, kLanes lanes per row, so that a request
+        // touches few lines; thread `lane` then looks after row `lane`.
+        constexpr int kLanes = D / 8, kStep = 32 / kLanes, kLoads = 32 / kStep;
+        const int chunk = lane % kLanes, sub = lane / kLanes, row0 = row - lane;
+        while (ok && advance_warp()) {
             const int r = 128 * i + row, pair = seg.rb * kBlockRows + r;
             const bool real = r < seg.rows;
-            const int token = real ? pair / p.group : 0;
-            // this thread's query row into the operand tile
+            const int token = real ? div(pair, p.group) : 0;
+            // the query row into the operand tile (its last products are done: this row tile's output was waited for)
             float c_row = fabsf(p.scale_log2e);
             {
                 const bool negate = p.scale_log2e < 0.f;   // scores are compared as they come, so their factor is kept positive
-                const bf16 *qp = p.q + (long long)(seg.first + token) * p.q_token + (long long)(seg.head * p.group + (real ? pair % p.group : 0)) * p.q_head;
-                uint4 raw[D / 8];
+                int e_row = 0;
+                uint4 raw[kLoads];
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) raw[c] = real ? __ldg(reinterpret_cast<const uint4 *>(qp) + c) : make_uint4(0u, 0u, 0u, 0u);
-                float factor = negate ? -1.f : 1.f;
-                if constexpr (FP8) {
-                    float amax = 0.f;
+                for (int it = 0; it < kLoads; ++it) {
+                    const int rr = 128 * i + row0 + it * kStep + sub, pr = seg.rb * kBlockRows + rr, tk = div(pr, p.group);
+                    const bf16 *qp = p.q + (long long)(seg.first + tk) * p.q_token + (long long)(seg.head * p.group.d + pr - tk * p.group.d) * p.q_head;
+                    raw[it] = rr < seg.rows ? __ldg(reinterpret_cast<const uint4 *>(qp) + chunk) : make_uint4(0u, 0u, 0u, 0u);
+                }
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        float x[8];
-                        unpack8(raw[c], x);
+                for (int it = 0; it < kLoads; ++it) {
+                    uint4 w = raw[it];
+                    if constexpr (FP8) {
+                        float x[8], amax = 0.f;
+                        unpack8(raw[it], x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const float a = fabsf(x[k]);
                             if (a < INFINITY) amax = fmaxf(amax, a);
                         }
-                    }
-                    const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120);   // amax / 2^e in [2^14, 2^15)
-                    factor *= __uint_as_float((uint32_t)(127 - e) << 23);
-                    c_row *= __uint_as_float((uint32_t)(127 + e) << 23);
-                }
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 w = raw[c];
-                    if constexpr (FP8) {
-                        float x[8];
-                        unpack8(raw[c], x);
+                        for (int off = kLanes / 2; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+                        const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120);   // amax / 2^e in [2^14, 2^15)
+                        const float factor = __uint_as_float((uint32_t)(127 - e) << 23) * (negate ? -1.f : 1.f);
                         w = make_uint4(pack_f16(x[0] * factor, x[1] * factor), pack_f16(x[2] * factor, x[3] * factor),
                                        pack_f16(x[4] * factor, x[5] * factor), pack_f16(x[6] * factor, x[7] * factor));
+                        const int mine = __shfl_sync(0xffffffffu, e, (lane % kStep) * kLanes);
+                        if (lane / kStep == it) e_row = mine;
                     } else if (negate) {
                         w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u;
                     }
-                    *reinterpret_cast<uint4 *>(s.q[i] + operand_chunk(row, c)) = w;
+                    *reinterpret_cast<uint4 *>(s.q[i] + operand_chunk(row0 + it * kStep + sub, chunk)) = w;
                 }
+                if constexpr (FP8) c_row *= __uint_as_float((uint32_t)(127 + e_row) << 23);
                 fence_async_smem();
-                mbar_arrive(&s.q_full);
+                mbar_arrive(&s.q_full[i]);
             }
             const int limit = real ? visible(seg.length, seg.count, token) : 0;
-            const int all_see = visible(seg.length, seg.count, (seg.rb * kBlockRows + 128 * i) / p.group);
+            const int all_see = visible(seg.length, seg.count, div(seg.rb * kBlockRows + 128 * i, p.group));
             float m = -INFINITY, l = 0.f;
-            const int n = seg.n[i], n_any = max(seg.n[0], seg.n[1]);
+            const int n = shape.n[i];
 
             for (int j = 0; j < n; ++j) {
                 ok = __all_sync(0xffffffffu, wait_bar(&s.s_full[i], s_parity, failed));
@@ -337,150 +321,162 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 const int slot = (tile_ctr + j) & 3, pos0 = (seg.tile0 + j) * kTileTokens;
                 const bool masked = pos0 + kTileTokens > all_see;
                 const int lim = limit - pos0;   // columns below it are seen
-                const bool general = FP8 || s.general[slot] != 0;
-                uint32_t x[2][32];
-
-                // largest score
-                float top = -INFINITY;
-                tmem_load32(s_tm, x[0]);
+                uint32_t x[4][32];
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) tmem_load32(s_tm + 32 * ch, x[ch]);
                 tmem_load_wait(x[0]);
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    if (ch < 3) tmem_load32(s_tm + 32 * (ch + 1), x[(ch + 1) & 1]);
+                for (int ch = 1; ch < 4; ++ch) after_wait(x[ch]);
+                if (masked) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float c = general ? c_row * s.ks[slot][2 * ch + h] : c_row;
-                        const float e = general ? s.ev[slot][2 * ch + h] : 0.f;
-                        if (masked) {
+                    for (int k = 0; k < 128; ++k)
+                        if (k >= lim) x[k / 32][k % 32] = 0xff800000u;   // -inf
+                }
+                // largest score; 16 positions share a page and so a key scale c and a value scale 2^e.  NaN stays NaN, and
+                // with it the row.
+                float top = -INFINITY;
 #pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                top = fmaxf(top, 32 * ch + 16 * h + k < lim ? fmaf(__uint_as_float(x[ch & 1][16 * h + k]), c, e) : -INFINITY);
-                        } else {
-                            float mx = __uint_as_float(x[ch & 1][16 * h]);
+                for (int h = 0; h < 8; ++h) {
+                    const uint32_t *y = &x[h / 2][16 * (h & 1)];
+                    float a = __uint_as_float(y[0]), b = __uint_as_float(y[1]);
 #pragma unroll
-                            for (int k = 1; k < 16; ++k) mx = fmaxf(mx, __uint_as_float(x[ch & 1][16 * h + k]));
-                            top = fmaxf(top, fmaf(mx, c, e));
-                        }
+                    for (int k = 2; k < 14; k += 4) {
+                        a = max3_nan(a, __uint_as_float(y[k]), __uint_as_float(y[k + 1]));
+                        b = max3_nan(b, __uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
                     }
-                    if (ch < 3) tmem_load_wait(x[(ch + 1) & 1]);
+                    a = max3_nan(max3_nan(a, __uint_as_float(y[14]), __uint_as_float(y[15])), b, b);
+                    top = max3_nan(top, top, fmaf(a, fmaxf(c_row * s.ks[slot][h], kLeastFactor), s.ev[slot][h]));
                 }
                 // the running maximum, and the output if it has grown too much
                 {
-                    const float grown = fmaxf(m, top);
+                    const float grown = max3_nan(m, m, top);
                     const bool need = grown > m + 8.f;   // also from -inf
                     if (j == 0) {
                         m = grown;
-                    } else if (__any_sync(0xffffffffu, need)) {
+                    } else if (__any_sync(0xffffffffu, need || grown != grown)) {
                         const float corr = need ? exp2_fast(m - grown) : 1.f;
-                        if (need) m = grown;
+                        if (need || grown != grown) m = grown;
                         l *= corr;
+#pragma unroll 1
+                        for (int ch = 0; ch < D / 16; ++ch) {
+                            uint32_t o[16];
+                            tmem_load16(o_tm + 16 * ch, o);
 #pragma unroll
-                        for (int ch = 0; ch < D / 32; ++ch) {
-                            tmem_load32(o_tm + 32 * ch, x[0]);
-                            tmem_load_wait(x[0]);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) x[0][k] = __float_as_uint(__uint_as_float(x[0][k]) * corr);
-                            tmem_store32(o_tm + 32 * ch, x[0]);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                            tmem_store16(o_tm + 16 * ch, o);
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                // weights, in the place of the scores
-                tmem_load32(s_tm, x[0]);
-                tmem_load_wait(x[0]);
+                const float base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : m;
+                // weights, in the place of the scores, in two halves: the first one's product runs under the second's exponentials
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
-                    if (ch < 3) tmem_load32(s_tm + 32 * (ch + 1), x[(ch + 1) & 1]);
                     uint32_t w[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float c = general ? c_row * s.ks[slot][2 * ch + h] : c_row;
-                        const float e = (general ? s.ev[slot][2 * ch + h] : 0.f) - base;
-                        float sum0 = 0.f, sum1 = 0.f;
+                        const float c = fmaxf(c_row * s.ks[slot][2 * ch + h], kLeastFactor), e = s.ev[slot][2 * ch + h] - base;
+                        const uint64_t cc = pair_f32(c, c), ee = pair_f32(e, e);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            float w0 = exp2_fast(fmaf(__uint_as_float(x[ch & 1][16 * h + k]), c, e));
-                            float w1 = exp2_fast(fmaf(__uint_as_float(x[ch & 1][16 * h + k + 1]), c, e));
-                            if (masked) {
-                                if (32 * ch + 16 * h + k >= lim) w0 = 0.f;
-                                if (32 * ch + 16 * h + k + 1 >= lim) w1 = 0.f;
+                            const uint64_t z = fma_f32x2(pair_f32(__uint_as_float(x[ch][16 * h + k]), __uint_as_float(x[ch][16 * h + k + 1])), cc, ee);
+                            float w0, w1;
+                            if (k % 8 < kPolynomialOf8) {   // on the fused multiply-add pipe, the others on the special function unit
+                                split_f32(exp2_polynomial(z), w0, w1);
+                            } else {
+                                split_f32(z, w0, w1);
+                                w0 = exp2_fast(w0);
+                                w1 = exp2_fast(w1);
                             }
-                            sum0 += w0;
-                            sum1 += w1;
+                            sum = add_f32x2(sum, pair_f32(w0, w1));
                             w[8 * h + k / 2] = FP8 ? pack_f16(w0, w1) : pack_b16(w0, w1);
                         }
-                        l = general ? fmaf(sum0 + sum1, s.iev[slot][2 * ch + h], l) : l + (sum0 + sum1);
+                        float s0, s1;
+                        split_f32(sum, s0, s1);
+                        l = fmaf(s0 + s1, s.iev[slot][2 * ch + h], l);
                     }
-                    if (ch < 3) tmem_load_wait(x[(ch + 1) & 1]);   // a store only overwrites columns that have been read
                     tmem_store16(s_tm + 16 * ch, w);
+                    if (ch & 1) {
+                        tmem_store_wait();
+                        tcgen05_fence_before();
+                        mbar_arrive(&s.p_full[i][ch >> 1]);
+                    }
                 }
-                tmem_store_wait();
-                tcgen05_fence_before();
-                mbar_arrive(&s.p_full[i]);
             }
-            tile_ctr += n_any;
+            tile_ctr += shape.most;
             if (!ok) break;
 
-            // epilogue
             ok = __all_sync(0xffffffffu, wait_bar(&s.o_full[i], o_parity, failed));
             if (!ok) break;
             o_parity ^= 1u;
             tcgen05_fence_after();
             const int buffer = bearing & (kBadBuffers - 1);
             const bool bad = n > 0 && (volatile int &)s.bad_any[buffer] != 0;
-            if (n_any > 0) ++bearing;
+            if (shape.most > 0) ++bearing;
+            const bool complete = seg.begins && seg.ends;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            float *part = p.partial + ((long long)blockIdx.x * 2 + (seg.tile0 == 0 ? 1 : 0)) * kBlockRows * (D + 2);
-            bf16 *dst = p.out + ((long long)(seg.first + token) * p.hq + seg.head * p.group + (real ? pair % p.group : 0)) * D;
-#pragma unroll 1
-            for (int ch = 0; ch < D / 32; ++ch) {
-                uint32_t x[32];
-                if (n > 0) {
-                    tmem_load32(o_tm + 32 * ch, x);
-                    tmem_load_wait(x);
-                } else {
+            float *part = p.partial + ((long long)blockIdx.x * 2 + (seg.begins ? 1 : 0)) * kBlockRows * (D + 2);
+            uint32_t x[D / 32][32];
+            if (n > 0) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = 0u;
-                }
-                if (bad) {
+                for (int ch = 0; ch < D / 32; ++ch) tmem_load32(o_tm + 32 * ch, x[ch]);
+                tmem_load_wait(x[0]);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        float y = __uint_as_float(x[k]);
-                        if ((volatile int &)s.bad[buffer][0][32 * ch + k] < limit) y = __int_as_float(0x7fffffff);
-                        if constexpr (!FP8) {
-                            if ((volatile int &)s.bad[buffer][1][32 * ch + k] < limit) y += INFINITY;
-                            if ((volatile int &)s.bad[buffer][2][32 * ch + k] < limit) y -= INFINITY;
-                        }
-                        x[k] = __float_as_uint(y);
+                for (int ch = 1; ch < D / 32; ++ch) after_wait(x[ch]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < D; ++k) x[k / 32][k % 32] = 0u;
+            }
+            if (bad) {
+#pragma unroll
+                for (int k = 0; k < D; ++k) {
+                    float y = __uint_as_float(x[k / 32][k % 32]);
+                    if ((volatile int &)s.bad[buffer][0][k] < limit) y = __int_as_float(0x7fffffff);
+                    if constexpr (!FP8) {
+                        if ((volatile int &)s.bad[buffer][1][k] < limit) y += INFINITY;
+                        if ((volatile int &)s.bad[buffer][2][k] < limit) y -= INFINITY;
                     }
-                }
-                if (real) {
-                    if (seg.complete) {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            uint4 v;
-                            v.x = pack_b16(__uint_as_float(x[k]) * inv, __uint_as_float(x[k + 1]) * inv);
-                            v.y = pack_b16(__uint_as_float(x[k + 2]) * inv, __uint_as_float(x[k + 3]) * inv);
-                            v.z = pack_b16(__uint_as_float(x[k + 4]) * inv, __uint_as_float(x[k + 5]) * inv);
-                            v.w = pack_b16(__uint_as_float(x[k + 6]) * inv, __uint_as_float(x[k + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(dst + 32 * ch + k) = v;
-                        }
-                    } else {   // four columns of 256 rows side by side
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            *reinterpret_cast<uint4 *>(part + ((32 * ch + k) / 4 * kBlockRows + r) * 4) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-                    }
+                    x[k / 32][k % 32] = __float_as_uint(y);
                 }
             }
-            if (real && !seg.complete) *reinterpret_cast<float2 *>(part + D * kBlockRows + 2 * r) = make_float2(m, l);
+            if (complete) {   // through the query tile, which is idle now, to whole lines of the output
+#pragma unroll
+                for (int k = 0; k < D; k += 8) {
+                    const uint32_t *y = &x[k / 32][k % 32];
+                    uint4 v;
+                    v.x = pack_b16(__uint_as_float(y[0]) * inv, __uint_as_float(y[1]) * inv);
+                    v.y = pack_b16(__uint_as_float(y[2]) * inv, __uint_as_float(y[3]) * inv);
+                    v.z = pack_b16(__uint_as_float(y[4]) * inv, __uint_as_float(y[5]) * inv);
+                    v.w = pack_b16(__uint_as_float(y[6]) * inv, __uint_as_float(y[7]) * inv);
+                    *reinterpret_cast<uint4 *>(s.q[i] + operand_chunk(row, k / 8)) = v;
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int it = 0; it < kLoads; ++it) {
+                    const int rr = row0 + it * kStep + sub, pr = seg.rb * kBlockRows + 128 * i + rr, tk = div(pr, p.group);
+                    if (128 * i + rr < seg.rows)
+                        *reinterpret_cast<uint4 *>(p.out + ((long long)(seg.first + tk) * p.hq + seg.head * p.group.d + pr - tk * p.group.d) * D + 8 * chunk) =
+                            *reinterpret_cast<const uint4 *>(s.q[i] + operand_chunk(rr, chunk));
+                }
+                __syncwarp();
+            } else if (real) {   // four columns of 256 rows side by side
+#pragma unroll
+                for (int k = 0; k < D; k += 4) {
+                    const uint32_t *y = &x[k / 32][k % 32];
+                    *reinterpret_cast<uint4 *>(part + (k / 4 * kBlockRows + r) * 4) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            if (real && !complete) *reinterpret_cast<float2 *>(part + D * kBlockRows + 2 * r) = make_float2(m, l);
         }
-    } else if (warp == 8) {
+    } else {
+    give_up_registers<T::kOtherRegisters>();
+    if (warp == 8) {
         // ------------------------------------------------------------------ loader
         uint32_t kv_it = 0, raw_stage = 0, raw_parity = 0, raw_fills = 0, v_raw_parity = 0;
         int bearing = 0;
         bool ok = true;
-        while (ok && walk.next(pp, seg)) {
-            const int n = max(seg.n[0], seg.n[1]);
+        while (ok && advance_warp()) {
+            const int n = shape.most;
             if (n == 0) continue;
             const int buffer = bearing & (kBadBuffers - 1);
             ++bearing;
@@ -488,36 +484,39 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (lane == 0) s.bad_any[buffer] = 0;
             __syncwarp();
             const int *table = bt.table + seg.b * bt.table_stride;
-            // page of 16-position chunk `lane` of a tile
-            auto page_of = [&](int j) {
+            // table entry of 16-position chunk `lane` of a tile; used, and checked, two tiles later
+            auto entry_of = [&](int j) {
                 const int pos = (seg.tile0 + j) * kTileTokens + 16 * lane;
-                if (lane >= kChunks || j >= n || pos >= seg.length) return -1;
-                const int id = __ldg(table + (pos >> bt.page_shift));
-                if (id >= bt.num_pages) {
-                    atomicOr(bt.error, kErrorIndex);
-                    return -1;
-                }
-                return id < 0 ? -1 : id;
+                return lane < kChunks && j < n && pos < seg.length ? __ldg(table + (pos >> bt.page_shift)) : -1;
             };
-            int page = page_of(0);
+            auto checked = [&](int id) {
+                if (id >= bt.num_pages) atomicOr(bt.error, kErrorIndex);
+                return id >= 0 && id < bt.num_pages ? id : -1;
+            };
+            // scales of a tile's pages, as they lie in memory
+            auto scales_of = [&](int id, float &ks, float &vs) {
+                ks = 1.f;
+                vs = 1.f;
+                if (FP8 && id >= 0) {
+                    const long long at = (long long)id * p.hkv + seg.head;
+                    ks = __ldg(p.k_scales + at);
+                    vs = __ldg(p.v_scales + at);
+                }
+            };
+            // page ids are fetched two tiles ahead, scales one
+            int page = entry_of(0), page_next = entry_of(1);
+            page = checked(page);
+            float ks_raw, vs_raw;
+            scales_of(page, ks_raw, vs_raw);
             for (int j = 0; j < n; ++j, ++kv_it) {
-                const int page_next = page_of(j + 1);
+                const int page_after = entry_of(j + 2);
+                page_next = checked(page_next);
+                float ks_next, vs_next;
+                scales_of(page_next, ks_next, vs_next);
                 const int pos0 = (seg.tile0 + j) * kTileTokens, stage = kv_it & 1, slot = kv_it & 3;
                 const uint32_t reuse = ((kv_it >> 1) & 1) ^ 1u;   // parity of the stage's last release
-                float ks = 1.f, ev = -INFINITY, iev = 0.f;
-                if (lane < kChunks && page >= 0) {
-                    ev = 0.f;
-                    iev = 1.f;
-                    if constexpr (FP8) {
-                        const long long at = (long long)page * p.hkv + seg.head;
-                        const float vs = fmaxf(__ldg(p.v_scales + at), 0x1p-100f);
-                        ks = __ldg(p.k_scales + at);
-                        ev = log2f(vs);
-                        iev = 1.f / vs;
-                    }
-                }
-                const bool behind_end = pos0 + 16 * lane >= seg.length;
-                const bool general = __any_sync(0xffffffffu, lane < kChunks && page < 0 && !behind_end);
+                const float vs = fmaxf(vs_raw, 0x1p-100f), ks = ks_raw;
+                const float ev = page < 0 ? -INFINITY : FP8 ? log2f(vs) : 0.f, iev = page < 0 ? 0.f : FP8 ? 1.f / vs : 1.f;
 
                 // positions [from, from + tokens) of the tile; all lanes call it, lane 0 issues
                 auto boxes = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, int from, int tokens) {
@@ -541,7 +540,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         if (!ok) break;
                         if (part == 0) {   // before the barrier that leads to this tile's scores
                             if (lane < kChunks) { s.ks[slot][lane] = ks; s.ev[slot][lane] = ev; s.iev[slot][lane] = iev; }
-                            if (lane == 0) s.general[slot] = 1;
                             __syncwarp();
                         }
                         if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[raw_stage], T::kRawBytes);
@@ -555,14 +553,13 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     ok = __all_sync(0xffffffffu, wait_bar(&s.k_empty[stage], reuse, failed));
                     if (!ok) break;
                     if (lane < kChunks) { s.ks[slot][lane] = ks; s.ev[slot][lane] = ev; s.iev[slot][lane] = iev; }
-                    if (lane == 0) s.general[slot] = general ? 1 : 0;
                     __syncwarp();
                     if (lane == 0) mbar_arrive_expect_tx(&s.k_full[stage], T::kOperandBytes);
                     __syncwarp();
                     boxes(s.k[stage], &map_k, &s.k_full[stage], 0, kTileTokens);
                     ok = __all_sync(0xffffffffu, wait_bar(&s.v_empty[stage], reuse, failed));
                     if (!ok) break;
-                    const bool edge = pos0 + kTileTokens > seg.all_see;   // some rows do not see all of it
+                    const bool edge = pos0 + kTileTokens > shape.all_see;   // some rows do not see all of it
                     uint64_t *bar = edge ? &s.v_raw : &s.v_full[stage];
                     if (lane == 0) mbar_arrive_expect_tx(bar, T::kOperandBytes);
                     __syncwarp();
@@ -571,38 +568,43 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         ok = __all_sync(0xffffffffu, wait_bar(&s.v_raw, v_raw_parity, failed));
                         if (!ok) break;
                         v_raw_parity ^= 1u;
-                        const int from = max(seg.all_see - pos0, 0);
-                        for (int idx = from * (D / 8) + lane; idx < kTileTokens * (D / 8); idx += 32) {
-                            const int r = idx / (D / 8), c = idx % (D / 8);
-                            uint4 *at = reinterpret_cast<uint4 *>(s.v[stage] + operand_chunk(r, c));
-                            if (pos0 + r >= seg.length) {
-                                *at = make_uint4(0u, 0u, 0u, 0u);
-                            } else {
+                        const int from = max(shape.all_see - pos0, 0), end = min(max(seg.length - pos0, 0), kTileTokens);
+                        // anything that is not finite among the positions that only some rows see?
+                        uint32_t odd = 0;
+#pragma unroll 8
+                        for (int idx = from * (D / 8) + lane; idx < end * (D / 8); idx += 32) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(s.v[stage] + operand_chunk(idx / (D / 8), idx % (D / 8)));
+                            odd |= not_finite_b16(v.x) | not_finite_b16(v.y) | not_finite_b16(v.z) | not_finite_b16(v.w);
+                        }
+                        if (__any_sync(0xffffffffu, odd != 0)) {
+                            for (int idx = from * (D / 8) + lane; idx < end * (D / 8); idx += 32) {
+                                const int r = idx / (D / 8), c = idx % (D / 8);
+                                uint4 *at = reinterpret_cast<uint4 *>(s.v[stage] + operand_chunk(r, c));
                                 const uint4 v = *at;
                                 uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                                uint32_t odd = 0;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) odd |= __vcmpeq2(w[k] & 0x7f807f80u, 0x7f807f80u);
-                                if (odd) {
-#pragma unroll
-                                    for (int k = 0; k < 8; ++k) {
-                                        const uint32_t bits = (w[k / 2] >> (16 * (k & 1))) & 0xffffu;
-                                        if ((bits & 0x7f80u) == 0x7f80u) {
-                                            atomicMin(&s.bad[buffer][(bits & 0x7fu) ? 0 : (bits & 0x8000u) ? 2 : 1][8 * c + k], pos0 + r);
-                                            w[k / 2] &= ~(0xffffu << (16 * (k & 1)));
-                                        }
+                                for (int k = 0; k < 8; ++k) {
+                                    const uint32_t bits = (w[k / 2] >> (16 * (k & 1))) & 0xffffu;
+                                    if ((bits & 0x7f80u) == 0x7f80u) {
+                                        atomicMin(&s.bad[buffer][(bits & 0x7fu) ? 0 : (bits & 0x8000u) ? 2 : 1][8 * c + k], pos0 + r);
+                                        w[k / 2] &= ~(0xffffu << (16 * (k & 1)));
                                     }
-                                    s.bad_any[buffer] = 1;
-                                    *at = make_uint4(w[0], w[1], w[2], w[3]);
                                 }
+                                *at = make_uint4(w[0], w[1], w[2], w[3]);
                             }
+                            s.bad_any[buffer] = 1;
                         }
+                        for (int idx = end * (D / 8) + lane; idx < kTileTokens * (D / 8); idx += 32)   // behind the end: anything may lie there
+                            *reinterpret_cast<uint4 *>(s.v[stage] + operand_chunk(idx / (D / 8), idx % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&s.v_full[stage]);
                     }
                 }
                 page = page_next;
+                page_next = page_after;
+                ks_raw = ks_next;
+                vs_raw = vs_next;
             }
         }
         // Never leave with copies in flight: in a clean run the other roles have waited for every fill.
@@ -622,76 +624,112 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
-        // ------------------------------------------------------------------ MMA issue
+    } else if (warp == 9 || warp == 10) {
+        // ------------------------------------------------------------------ MMA issue for one row tile
         if (lane == 0) {
+            const int i = warp - 9;
             const uint32_t idesc_s = umma_idesc16(!FP8, kTileTokens, false), idesc_o = umma_idesc16(!FP8, D, true);
-            uint32_t kv_it = 0, q_parity = 0, p_parity[2] = {0u, 0u};
+            const uint32_t s_tm = tmem + i * 128, o_tm = tmem + 256 + i * 128;
+            uint32_t kv_it = 0, q_parity = 0, p_parity = 0;
             bool ok = true;
-            auto scores = [&](int i, uint32_t it) {   // S_i = Q_i K^T
-                const uint64_t dq = smem_desc_k_major_sw128(s.q[i]), dk = smem_desc_k_major_sw128(s.k[it & 1]);
+            const uint64_t dq = smem_desc_k_major_sw128(s.q[i]), dk0 = smem_desc_k_major_sw128(s.k[0]);
+            const uint64_t dv0 = smem_desc_mn_major_sw128(s.v[0], kPanelBytes);
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                ok = ok && wait_bar(bar, parity, failed);
+                return ok;
+            };
+            // S = Q K^T of tile t (or, where this row tile has no use for it, only the stage's release)
+            auto scores = [&](uint32_t t, bool used) {
+                if (!wait(&s.k_full[t & 1], (t >> 1) & 1)) return;
+                if (!used) {
+                    mbar_arrive(&s.k_empty[t & 1]);
+                    return;
+                }
+                tcgen05_fence_after();
+                const uint64_t dk = dk0 + (t & 1) * (T::kOperandBytes >> 4);
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint64_t step = (uint64_t)((ks >> 2) * (kPanelBytes >> 4) + (ks & 3) * 2);
-                    umma16_ss(tmem + i * 128, dq + step, dk + step, idesc_s, ks != 0);
+                    const uint64_t at = (uint64_t)((ks >> 2) * (kPanelBytes >> 4) + (ks & 3) * 2);
+                    umma16_ss(s_tm, dq + at, dk + at, idesc_s, ks != 0);
                 }
                 umma_commit(&s.s_full[i]);
+                umma_commit(&s.k_empty[t & 1]);
             };
-            while (ok && walk.next(pp, seg)) {
-                if (!(ok = wait_bar(&s.q_full, q_parity, failed))) break;
+            while (ok && advance(true)) {
+                if (!wait(&s.q_full[i], q_parity)) break;
                 q_parity ^= 1u;
-                const int n = max(seg.n[0], seg.n[1]);
-                for (int i = 0; i < 2; ++i)   // a row tile without positions goes on, but never ahead of this segment
-                    if (seg.n[i] == 0) mbar_arrive(&s.o_full[i]);
-                if (n == 0) continue;
-                if (!(ok = wait_bar(&s.k_full[kv_it & 1], (kv_it >> 1) & 1, failed))) break;
-                tcgen05_fence_after();
-                for (int i = 0; i < 2; ++i)
-                    if (seg.n[i] > 0) scores(i, kv_it);
-                umma_commit(&s.k_empty[kv_it & 1]);
-                for (int j = 0; ok && j < n; ++j, ++kv_it) {
-                    if (!(ok = wait_bar(&s.v_full[kv_it & 1], (kv_it >> 1) & 1, failed))) break;
-                    if (j + 1 < n && !(ok = wait_bar(&s.k_full[(kv_it + 1) & 1], ((kv_it + 1) >> 1) & 1, failed))) break;
-                    const uint64_t dv = smem_desc_mn_major_sw128(s.v[kv_it & 1], kPanelBytes);
-                    for (int i = 0; i < 2; ++i) {
-                        if (j >= seg.n[i]) continue;
-                        if (!(ok = wait_bar(&s.p_full[i], p_parity[i], failed))) break;
-                        p_parity[i] ^= 1u;
-                        tcgen05_fence_after();
+                const int n = shape.n[i];
+                if (n == 0) mbar_arrive(&s.o_full[i]);
+                if (shape.most == 0) continue;
+                scores(kv_it, n > 0);
+                for (int j = 0; ok && j < shape.most; ++j, ++kv_it) {
+                    const uint32_t stage = kv_it & 1;
+                    if (!wait(&s.v_full[stage], (kv_it >> 1) & 1)) break;
+                    if (j < n) {   // a tile's weights come in halves
+                        const uint64_t dv = dv0 + stage * (T::kOperandBytes >> 4);
 #pragma unroll
-                        for (int ks = 0; ks < kTileTokens / 16; ++ks)   // 16 positions: 16 rows of 128 bytes, 8 columns of weights
-                            umma16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * ks, dv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j | ks) != 0);
-                        if (j + 1 < seg.n[i]) scores(i, kv_it + 1);
-                        else umma_commit(&s.o_full[i]);
+                        for (int half = 0; half < 2; ++half) {
+                            if (!wait(&s.p_full[i][half], p_parity)) break;
+                            tcgen05_fence_after();
+#pragma unroll
+                            for (int ks = 4 * half; ks < 4 * half + 4; ++ks)   // 16 positions: 16 rows of 128 bytes, 8 columns of weights
+                                umma16_ts(o_tm, s_tm + 8 * ks, dv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j | ks) != 0);
+                        }
+                        if (!ok) break;
+                        p_parity ^= 1u;
+                        if (j + 1 == n) umma_commit(&s.o_full[i]);
+                        umma_commit(&s.v_empty[stage]);
+                    } else {
+                        mbar_arrive(&s.v_empty[stage]);
                     }
-                    if (!ok) break;
-                    umma_commit(&s.v_empty[kv_it & 1]);
-                    if (j + 1 < n) umma_commit(&s.k_empty[(kv_it + 1) & 1]);
+                    if (j + 1 < shape.most) scores(kv_it + 1, j + 1 < n);
                 }
             }
             if (*failed) {   // products in flight still write tensor memory and read shared memory
-                umma_commit(&s.drain);
+                umma_commit(&s.drain[i]);
                 const long long began = clock64();
-                while (!mbar_try_wait(&s.drain, 0) && clock64() - began < kWaitCycles) {}
+                while (!mbar_try_wait(&s.drain[i], 0) && clock64() - began < kWaitCycles) {}
             }
         }
         __syncwarp();
-    } else if constexpr (FP8) {
+    } else if (warp == 11) {
+        // ------------------------------------------------------------------ planner
+        if (lane == 0) {
+            JoinEntry entry = {0, 0, 0, 0};
+            bool more = true;
+            while (more) {
+                more = next_segment(bt, p.hkv, p.group, kPrefillCut, walk, seg);
+                if (more) {
+                    shape = shape_of(p, seg);
+                    if (seg.parts > 1) entry = JoinEntry{seg.parts, seg.first, seg.rb * kBlockRows, (seg.head << 16) | seg.rows};
+                }
+                const int at = orders & (kOrders - 1);
+                if (!wait_bar(&s.order_empty[at], ((orders / kOrders) & 1) ^ 1u, failed)) break;
+                s.order[at].seg = seg;
+                s.order[at].shape = shape;
+                s.order[at].valid = more ? 1 : 0;
+                mbar_arrive(&s.order_full[at]);
+                ++orders;
+            }
+            p.entries[blockIdx.x] = entry;
+        }
+        __syncwarp();
+    } else if (FP8 && warp >= 12) {
         // ------------------------------------------------------------------ converters
-        const int tid = threadIdx.x - 320;
+        const int tid = threadIdx.x - 384;
         constexpr int kPerRow = D / 16, kPer = T::kRawTokens * kPerRow / T::kConverters;   // 16-code chunks per row, per thread
         uint32_t kv_it = 0, raw_stage = 0, raw_parity = 0;
         int bearing = 0;
         bool ok = true;
-        while (ok && walk.next(pp, seg)) {
-            const int n = max(seg.n[0], seg.n[1]);
+        while (ok && advance_warp()) {
+            const int n = shape.most;
             if (n == 0) continue;
             const int buffer = bearing & (kBadBuffers - 1);
             ++bearing;
             for (int j = 0; ok && j < n; ++j, ++kv_it) {
                 const int pos0 = (seg.tile0 + j) * kTileTokens, stage = kv_it & 1;
                 const uint32_t reuse = ((kv_it >> 1) & 1) ^ 1u;
-                const bool edge = pos0 + kTileTokens > seg.all_see;
+                const bool edge = pos0 + kTileTokens > shape.all_see;
 #pragma unroll 1
                 for (int part = 0; part < 4; ++part) {
                     const bool is_v = part >= 2;
@@ -710,15 +748,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                             uint32_t w[4] = {codes[it].x, codes[it].y, codes[it].z, codes[it].w};
                             if (pos0 + r >= seg.length) {
                                 w[0] = w[1] = w[2] = w[3] = 0u;
-                            } else if (pos0 + r >= seg.all_see) {
+                            } else if (pos0 + r >= shape.all_see) {
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
-                                    const uint32_t odd = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                                    if (odd) {
+                                    if (not_finite_e4m3(w[k])) {
                                         for (int y = 0; y < 4; ++y)
-                                            if ((odd >> (8 * y)) & 1u) atomicMin(&s.bad[buffer][0][16 * c + 4 * k + y], pos0 + r);
+                                            if (((w[k] >> (8 * y)) & 0x7fu) == 0x7fu) {
+                                                atomicMin(&s.bad[buffer][0][16 * c + 4 * k + y], pos0 + r);
+                                                w[k] &= ~(0xffu << (8 * y));
+                                            }
                                         s.bad_any[buffer] = 1;
-                                        w[k] &= ~odd;
                                     }
                                 }
                             }
@@ -748,6 +787,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
         }
     }
+    }
 
     tcgen05_fence_before();
     __syncthreads();
@@ -758,57 +798,43 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     if (threadIdx.x == 0 && s.failed) atomicOr(bt.error, kErrorWait);
 }
 
-// Joins the parts of row blocks that several CTAs shared: one thread per row, a few columns per CTA.
+// Joins the parts of the row block that begins in CTA blockIdx.x's range, if there is one: one thread per
+// row, a few columns per CTA.
 constexpr int kJoinColumns = 16;
 template <int D>
 __global__ void __launch_bounds__(kBlockRows)
-join_blocks_kernel(const PrefillParams pp, int grid) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const AttentionParams &p = pp.a;
-    const Batch &bt = p.bt;
-    const int b = blockIdx.x, head = blockIdx.y, d0 = blockIdx.z * kJoinColumns, r = threadIdx.x;
-    const int u_seq = __ldg(p.prefix_out + b), units = __ldg(p.prefix_out + bt.seqs);
-    if (__ldg(p.prefix_out + b + 1) == u_seq) return;
-    const int ctas = working_ctas(grid, units);
-    int first, count;
-    rows_of(bt, b, first, count);
-    const int length = length_of(bt, b), blocks = block_count(count, p.group, kBlockRows);
-    int at = u_seq;
-    for (int rb = 0; rb < blocks; ++rb) {
-        const int tiles = max(block_tiles(length, count, p.group, kBlockRows, rb, kTileTokens), 1);
-        const int u0 = at + head * tiles, u1 = u0 + tiles;
-        at += tiles * p.hkv;
-        const int c0 = owner(u0, ctas, units), c1 = owner(u1 - 1, ctas, units);
-        if (c0 == c1 || r >= min(kBlockRows, count * p.group - rb * kBlockRows)) continue;
-        auto part_of = [&](int c) { return p.partial + ((long long)c * 2 + (c == c0 ? 1 : 0)) * kBlockRows * (D + 2); };
-        float top = -INFINITY;
-        for (int c = c0; c <= c1; ++c) top = fmaxf(top, part_of(c)[D * kBlockRows + 2 * r]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        float4 sum[kJoinColumns / 4];
+join_blocks_kernel(const AttentionParams p) {
+    pdl_wait();   // and no early start for the next kernel: see paged.cuh
+    const int4 raw = __ldg(reinterpret_cast<const int4 *>(p.entries + blockIdx.x));
+    const JoinEntry e = {raw.x, raw.y, raw.z, raw.w};
+    const int d0 = blockIdx.y * kJoinColumns, r = threadIdx.x, head = e.head_rows >> 16;
+    if (e.parts == 0 || r >= (e.head_rows & 0xffff)) return;
+    auto part_of = [&](int i) { return p.partial + ((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kBlockRows * (D + 2); };
+    float top = -INFINITY, total = 0.f;
+    float4 sum[kJoinColumns / 4];
 #pragma unroll
-        for (int k = 0; k < kJoinColumns / 4; ++k) sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < kJoinColumns / 4; ++k) sum[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
-        for (int c = c0; c <= c1; ++c) {
-            const float *src = part_of(c);
-            const float2 ml = *reinterpret_cast<const float2 *>(src + D * kBlockRows + 2 * r);
-            const float f = exp2_fast(ml.x - base);
-            total = fmaf(ml.y, f, total);
+    for (int i = 0; i < e.parts; ++i) {
+        const float *src = part_of(i);
+        const float2 ml = *reinterpret_cast<const float2 *>(src + D * kBlockRows + 2 * r);
+        const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
+        const float corr = exp2_fast(top - base), f = exp2_fast(ml.x - base);
+        top = now;
+        total = fmaf(total, corr, ml.y * f);
 #pragma unroll
-            for (int k = 0; k < kJoinColumns / 4; ++k) {
-                const float4 v = *reinterpret_cast<const float4 *>(src + ((d0 / 4 + k) * kBlockRows + r) * 4);
-                sum[k].x = fmaf(v.x, f, sum[k].x); sum[k].y = fmaf(v.y, f, sum[k].y);
-                sum[k].z = fmaf(v.z, f, sum[k].z); sum[k].w = fmaf(v.w, f, sum[k].w);
-            }
+        for (int k = 0; k < kJoinColumns / 4; ++k) {
+            const float4 v = *reinterpret_cast<const float4 *>(src + ((d0 / 4 + k) * kBlockRows + r) * 4);
+            sum[k].x = fmaf(sum[k].x, corr, v.x * f); sum[k].y = fmaf(sum[k].y, corr, v.y * f);
+            sum[k].z = fmaf(sum[k].z, corr, v.z * f); sum[k].w = fmaf(sum[k].w, corr, v.w * f);
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        const int pair = rb * kBlockRows + r;
-        bf16 *dst = p.out + ((long long)(first + pair / p.group) * p.hq + head * p.group + pair % p.group) * D + d0;
-#pragma unroll
-        for (int k = 0; k < kJoinColumns / 4; ++k)
-            bo::store_bf16x4(dst + 4 * k, make_float4(sum[k].x * inv, sum[k].y * inv, sum[k].z * inv, sum[k].w * inv));
     }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int pair = e.pair + r;
+    bf16 *dst = p.out + ((long long)(e.row + div(pair, p.group)) * p.hq + head * p.group.d + pair - div(pair, p.group) * p.group.d) * D + d0;
+#pragma unroll
+    for (int k = 0; k < kJoinColumns / 4; ++k)
+        bo::store_bf16x4(dst + 4 * k, make_float4(sum[k].x * inv, sum[k].y * inv, sum[k].z * inv, sum[k].w * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -822,30 +848,28 @@ PrefillGrid prefill_grid(const Pool &pool, const Batch &bt, int hq, int min_coun
     if (most < min_count) return g;   // no sequence can have as many rows
     const long long blocks = bt.cu ? (long long)bt.tokens * group / kBlockRows + bt.seqs : (long long)bt.seqs * block_count(bt.per_seq, group, kBlockRows);
     const long long tiles = (((long long)bt.max_pages << bt.page_shift) + kTileTokens - 1) / kTileTokens;
-    // Two row blocks per SM or more (counted by rows, not by what a ragged batch could have at worst): one CTA each.
-    g.whole = ((long long)bt.tokens * group / kBlockRows) * pool.kv_heads >= 2ll * sms || tiles == 1;
-    const long long units = blocks * pool.kv_heads * (g.whole ? 1 : tiles);
+    const long long units = blocks * pool.kv_heads * (tiles + kPrefillCost);
     g.too_many = units > 0x7fffffffll;
-    g.ctas = g.too_many ? 0 : g.whole || units < sms ? (int)units : sms;
-    g.partial_floats = g.whole ? 0 : (long long)g.ctas * 2 * kBlockRows * (pool.head_dim + 2);
+    g.ctas = g.too_many ? 0 : units < sms ? (int)units : sms;
+    g.partial_floats = (long long)g.ctas * 2 * kBlockRows * (pool.head_dim + 2);
     return g;
 }
 
 template <int D, bool FP8>
 static int launch_prefill_t(const PrefillParams &pp, const Pool &pool, const PrefillGrid &grid, cudaStream_t st) {
     using T = Prefill<D, FP8>;
+    using Smem = typename T::Smem;
     CUtensorMap map_k, map_v;
     const int most = FP8 ? T::kRawTokens : kTileTokens, box = pool.page_size < most ? pool.page_size : most;
     if (!make_pool_map(&map_k, pool, pool.k, box, !FP8) || !make_pool_map(&map_v, pool, pool.v, box, !FP8)) {
         set_last_error("mk_paged_attention: cuTensorMapEncodeTiled refused the cache (driver without tensor-map support?)");
         return MK_ERR_UNSUPPORTED;
     }
-    const size_t smem = 1024 + sizeof(typename T::Smem) + (size_t)(pp.a.bt.seqs + 1) * sizeof(int);
+    const size_t smem = offsetof(Smem, prefix) + (size_t)(pp.a.bt.seqs + 1) * sizeof(int);
     static bool allowed[64] = {};
     cudaError_t e = allow_smem((const void *)prefill_kernel<D, FP8>, allowed);
     if (e == cudaSuccess) e = launch_pdl(prefill_kernel<D, FP8>, dim3(grid.ctas), dim3(T::kThreads), smem, st, map_k, map_v, pp);
-    if (e == cudaSuccess && !grid.whole)
-        e = launch_pdl(join_blocks_kernel<D>, dim3(pp.a.bt.seqs, pp.a.hkv, D / kJoinColumns), dim3(kBlockRows), 0, st, pp, grid.ctas);
+    if (e == cudaSuccess) e = launch_pdl(join_blocks_kernel<D>, dim3(grid.ctas, D / kJoinColumns), dim3(kBlockRows), 0, st, pp.a);
     return (int)e;
 }
 
@@ -853,7 +877,6 @@ int launch_prefill(const AttentionParams &p, const Pool &pool, const PrefillGrid
     PrefillParams pp;
     pp.a = p;
     pp.min_count = min_count;
-    pp.whole = grid.whole ? 1 : 0;
     if (pool.head_dim == 64)
         return pool.fp8 ? launch_prefill_t<64, true>(pp, pool, grid, st) : launch_prefill_t<64, false>(pp, pool, grid, st);
     return pool.fp8 ? launch_prefill_t<128, true>(pp, pool, grid, st) : launch_prefill_t<128, false>(pp, pool, grid, st);
