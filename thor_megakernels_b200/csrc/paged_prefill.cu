@@ -1,20 +1,20 @@
 // Attention over a paged cache for sequences with many new rows (prompts, chunks of prompts):
 // the same operator as paged_attention.cu on the 5th-generation tensor cores.
 //
-// Shape of the work.  A row block is 256 (query token, query head of the group) pairs of one
-// sequence and KV head, two MMA tiles of 128 rows; the cache goes by in tiles of 128 positions.
-// Per tile and row tile:  S = Q K^T (tcgen05.mma, operands in shared memory, S in tensor memory),
+// Shape of the work.  A row block is 256 (token, query head of the group) pairs of one sequence and KV
+// head, two MMA tiles of 128 rows; the cache is loaded in tiles of 128 positions and worked off in steps of
+// 64.  Per step and row tile:  S = Q K^T (tcgen05.mma, operands in shared memory, S in tensor memory),
 // softmax weights P by one thread per row (tensor memory to registers and back, 16-bit), and
 // O += P V (P from tensor memory, V in shared memory as it lies there: positions are rows, so
 // it is an MN-major operand).  Everything a row needs is in one thread: no shuffles.
 //
-// What bounds it: per 128 x 128 tile the tensor core needs 4 x 128 x 128 x D flops - 1024 clocks
-// at D = 128 - and the softmax 128 x 128 exponentials - 1024 clocks of the special function unit.
-// Two row tiles alternate, so that one's softmax runs under the other's products:
-// S(j+1) follows O(j) in each row tile's order of issue, and weights take S's place in tensor memory, in
-// halves: the first half's product runs under the second half's exponentials.  The output is rescaled only when the running
-// maximum has grown by more than 2^8 since the last time (weights stay below 256, sums are fp32);
-// after the first tiles that is rare.
+// What bounds it: per 128 rows x 128 positions the tensor core needs 4 x 128 x 128 x D flops - 1024 clocks at
+// D = 128 - and the softmax 128 x 128 exponentials - 1024 clocks of the special function unit - and some 500
+// instructions per warp.  To keep a row tile's threads from waiting for its products, S has two
+// buffers of 64 columns per row tile: while one step's weights are made, the next step's scores are there
+// already, and the one after takes the place of the weights as soon as their product is done.  The output is
+// rescaled only when the running maximum has grown by more than 2^8 since the last time (weights stay below
+// 256, sums are fp32), and only then do the softmax threads wait for the product before.
 //
 // Warp roles: 0-3 and 4-7 softmax of row tile 0 and 1 (and query loading, epilogue), 8 loader (TMA,
 // one box per page), 9 and 10 MMA issue for one row tile each (9 also allocates tensor memory), 11 planner
@@ -50,20 +50,18 @@ void set_last_error(const char *msg);  // megakernel.cu
 
 namespace paged {
 
-constexpr int kTileTokens = 128;
+constexpr int kTileTokens = 128;           // positions that are loaded at once
+constexpr int kStepTokens = 64;            // positions of one product and softmax
 constexpr int kBlockRows = 256;
 constexpr int kPanelBytes = 128 * 128;     // 128 rows of one 128-byte swizzle row
 constexpr int kChunks = kTileTokens / 16;  // a page is at least 16 positions
 constexpr int kBadBuffers = 4;
-// 2^f, |f| <= 1/2: minimax in relative error (2.6e-6), found with the Remez exchange
-__device__ constexpr float kExp2[5] = {0.9999992847f, 0.6931217909f, 0.2402474433f, 0.0559178591f, 0.0095701022f};
-constexpr int kPolynomialOf8 = 2;          // of eight neighbouring exponentials, so many (pairs) are computed that way
 constexpr float kLeastFactor = 1.17549435e-38f;   // of a score: minus infinity (a masked score) times it stays what it is
 
 // What the roles need of a segment besides its place.
 struct Shape {
-    int n[2];           // tiles of the two row tiles in it
-    int most;           // the larger of them: tiles that are loaded
+    int n[2];           // steps (half tiles) of the two row tiles in it
+    int most;           // tiles that are loaded
     int all_see;        // positions that every row sees
 };
 // One segment as the planner hands it to the other roles.
@@ -94,7 +92,7 @@ struct Prefill {
         uint64_t raw_full[kRawStages], raw_empty[kRawStages], k_full[2], k_empty[2], v_full[2], v_empty[2], v_raw;
         uint64_t order_full[kOrders], order_empty[kOrders];
         Order order[kOrders];
-        uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drain[2];
+        uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], drain[2];   // [row tile], [row tile][step mod 2]
         float ks[4][kChunks], ev[4][kChunks], iev[4][kChunks];   // by tile counter mod 4: key scale, log2 of the value scale and its inverse
         int bad[kBadBuffers][kBadKinds][D];                      // first position whose value in a column is NaN, +inf, -inf
         int bad_any[kBadBuffers];
@@ -105,7 +103,7 @@ struct Prefill {
     };
 };
 
-constexpr int kPrefillCost = 2;            // of a segment besides its tiles, in tiles
+constexpr int kPrefillCost = 3;            // of a segment besides its tiles, in tiles
 __device__ constexpr Cut kPrefillCut = {kBlockRows, kTileTokens, kPrefillCost};
 
 struct PrefillParams {
@@ -122,10 +120,10 @@ __device__ __forceinline__ Shape shape_of(const AttentionParams &p, const Segmen
         h.n[i] = 0;
         if (last >= 128 * i) {
             const int seen = visible(s.length, s.count, div(s.rb * kBlockRows + last, p.group));
-            h.n[i] = max(min((seen + kTileTokens - 1) / kTileTokens, s.tile1) - s.tile0, 0);
+            h.n[i] = max(min((seen + kStepTokens - 1) / kStepTokens, 2 * s.tile1) - 2 * s.tile0, 0);
         }
     }
-    h.most = max(h.n[0], h.n[1]);
+    h.most = (max(h.n[0], h.n[1]) + 1) / 2;
     return h;
 }
 
@@ -149,23 +147,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float v;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
     return v;
-}
-
-// 2^x of a pair on the fused multiply-add pipe: x = n + f with n the nearest integer, 2^f (|f| <= 1/2) by a degree-4
-// polynomial, times 2^n put together from n's bits (0 from n = -127 down, so that what is not seen weighs nothing).
-__device__ __forceinline__ uint64_t exp2_polynomial(uint64_t x) {
-    float x0, x1;
-    split_f32(x, x0, x1);
-    x = pair_f32(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
-    const float magic = 12582912.f;   // 1.5 * 2^23: the sum's low bits are n
-    const uint64_t shifted = add_f32x2(x, pair_f32(magic, magic));
-    const uint64_t f = fma_f32x2(add_f32x2(shifted, pair_f32(-magic, -magic)), pair_f32(-1.f, -1.f), x);
-    uint64_t poly = pair_f32(kExp2[4], kExp2[4]);
-#pragma unroll
-    for (int k = 3; k >= 0; --k) poly = fma_f32x2(poly, f, pair_f32(kExp2[k], kExp2[k]));
-    float s0, s1;
-    split_f32(shifted, s0, s1);
-    return mul_f32x2(poly, pair_f32(__uint_as_float((__float_as_uint(s0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(s1) << 23) + 0x3f800000u)));
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -192,10 +173,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             mbar_init(&s.k_empty[i], 2);   // one arrival per row tile
             mbar_init(&s.v_empty[i], 2);
             mbar_init(&s.q_full[i], 128);
-            mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i][0], 128);
-            mbar_init(&s.p_full[i][1], 128);
-            mbar_init(&s.o_full[i], 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&s.s_full[i][h], 1);
+                mbar_init(&s.p_full[i][h], 128);
+                mbar_init(&s.o_done[i][h], 1);
+            }
         }
         for (int i = 0; i < T::kRawStages; ++i) {
             mbar_init(&s.raw_full[i], 1);
@@ -257,7 +239,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int i = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_tm = tmem + lanes + i * 128, o_tm = tmem + lanes + 256 + i * 128;
-        uint32_t s_parity = 0, o_parity = 0;
+        uint32_t s_parity = 0;           // bit h: of the scores of steps with that parity
+        uint32_t o_parity = 0;           // bit h: of the last product of steps with that parity, once it is asked for
+        // Waits for the product of the step before, the latest of its parity: one may be under way, not two, since the scores
+        // of a step follow the product two steps before it.
+        auto wait_output = [&](int h) {
+            const bool done = __all_sync(0xffffffffu, wait_bar(&s.o_done[i][h], ((o_parity >> h) & 1) ^ 1u, failed));
+            tcgen05_fence_after();
+            return done;
+        };
         int tile_ctr = 0, bearing = 0;   // tiles and tile-bearing segments of this CTA so far
         bool ok = true;
         // Queries: a warp loads its 32 rows side by side, kLanes lanes per row, so that a request
@@ -313,31 +303,34 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             float m = -INFINITY, l = 0.f;
             const int n = shape.n[i];
 
+#pragma unroll 1
             for (int j = 0; j < n; ++j) {
-                ok = __all_sync(0xffffffffu, wait_bar(&s.s_full[i], s_parity, failed));
+                const int h = j & 1;     // tile j / 2 of the segment, half h
+                ok = __all_sync(0xffffffffu, wait_bar(&s.s_full[i][h], (s_parity >> h) & 1, failed));
                 if (!ok) break;
-                s_parity ^= 1u;
+                s_parity ^= 1u << h;
                 tcgen05_fence_after();
-                const int slot = (tile_ctr + j) & 3, pos0 = (seg.tile0 + j) * kTileTokens;
-                const bool masked = pos0 + kTileTokens > all_see;
+                const int slot = (tile_ctr + j / 2) & 3, pos0 = (2 * seg.tile0 + j) * kStepTokens;
                 const int lim = limit - pos0;   // columns below it are seen
-                uint32_t x[4][32];
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) tmem_load32(s_tm + 32 * ch, x[ch]);
+                const uint32_t s_h = s_tm + h * kStepTokens;
+                uint32_t x[2][32];
+                tmem_load32(s_h, x[0]);
+                tmem_load32(s_h + 32, x[1]);
                 tmem_load_wait(x[0]);
+                after_wait(x[1]);
+                if (pos0 + kStepTokens > all_see) {
 #pragma unroll
-                for (int ch = 1; ch < 4; ++ch) after_wait(x[ch]);
-                if (masked) {
-#pragma unroll
-                    for (int k = 0; k < 128; ++k)
+                    for (int k = 0; k < kStepTokens; ++k)
                         if (k >= lim) x[k / 32][k % 32] = 0xff800000u;   // -inf
                 }
                 // largest score; 16 positions share a page and so a key scale c and a value scale 2^e.  NaN stays NaN, and
                 // with it the row.
-                float top = -INFINITY;
+                float c[4], e[4], top = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 8; ++h) {
-                    const uint32_t *y = &x[h / 2][16 * (h & 1)];
+                for (int g = 0; g < 4; ++g) {
+                    c[g] = fmaxf(c_row * s.ks[slot][4 * h + g], kLeastFactor);
+                    e[g] = s.ev[slot][4 * h + g];
+                    const uint32_t *y = &x[g / 2][16 * (g & 1)];
                     float a = __uint_as_float(y[0]), b = __uint_as_float(y[1]);
 #pragma unroll
                     for (int k = 2; k < 14; k += 4) {
@@ -345,17 +338,18 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         b = max3_nan(b, __uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
                     }
                     a = max3_nan(max3_nan(a, __uint_as_float(y[14]), __uint_as_float(y[15])), b, b);
-                    top = max3_nan(top, top, fmaf(a, fmaxf(c_row * s.ks[slot][h], kLeastFactor), s.ev[slot][h]));
+                    top = max3_nan(top, top, fmaf(a, c[g], e[g]));
                 }
                 // the running maximum, and the output if it has grown too much
                 {
                     const float grown = max3_nan(m, m, top);
-                    const bool need = grown > m + 8.f;   // also from -inf
+                    const bool need = !(grown <= m + 8.f);   // also from -inf, and NaN
                     if (j == 0) {
                         m = grown;
-                    } else if (__any_sync(0xffffffffu, need || grown != grown)) {
-                        const float corr = need ? exp2_fast(m - grown) : 1.f;
-                        if (need || grown != grown) m = grown;
+                    } else if (__any_sync(0xffffffffu, need)) {
+                        if (!(ok = wait_output(h ^ 1))) break;
+                        const float corr = need ? exp2_fast(m - (grown == -INFINITY ? 0.f : grown)) : 1.f;
+                        if (need) m = grown;
                         l *= corr;
 #pragma unroll 1
                         for (int ch = 0; ch < D / 16; ++ch) {
@@ -368,48 +362,41 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : m;
-                // weights, in the place of the scores, in two halves: the first one's product runs under the second's exponentials
+                // weights, in the place of the scores
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
+                for (int ch = 0; ch < 2; ++ch) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float c = fmaxf(c_row * s.ks[slot][2 * ch + h], kLeastFactor), e = s.ev[slot][2 * ch + h] - base;
-                        const uint64_t cc = pair_f32(c, c), ee = pair_f32(e, e);
+                    for (int half = 0; half < 2; ++half) {
+                        const int g = 2 * ch + half;
+                        const uint64_t cc = pair_f32(c[g], c[g]), ee = pair_f32(e[g] - base, e[g] - base);
                         uint64_t sum = 0;
 #pragma unroll
                         for (int k = 0; k < 16; k += 2) {
-                            const uint64_t z = fma_f32x2(pair_f32(__uint_as_float(x[ch][16 * h + k]), __uint_as_float(x[ch][16 * h + k + 1])), cc, ee);
                             float w0, w1;
-                            if (k % 8 < kPolynomialOf8) {   // on the fused multiply-add pipe, the others on the special function unit
-                                split_f32(exp2_polynomial(z), w0, w1);
-                            } else {
-                                split_f32(z, w0, w1);
-                                w0 = exp2_fast(w0);
-                                w1 = exp2_fast(w1);
-                            }
+                            split_f32(fma_f32x2(pair_f32(__uint_as_float(x[ch][16 * half + k]), __uint_as_float(x[ch][16 * half + k + 1])), cc, ee), w0, w1);
+                            w0 = exp2_fast(w0);
+                            w1 = exp2_fast(w1);
                             sum = add_f32x2(sum, pair_f32(w0, w1));
-                            w[8 * h + k / 2] = FP8 ? pack_f16(w0, w1) : pack_b16(w0, w1);
+                            w[8 * half + k / 2] = FP8 ? pack_f16(w0, w1) : pack_b16(w0, w1);
                         }
                         float s0, s1;
                         split_f32(sum, s0, s1);
-                        l = fmaf(s0 + s1, s.iev[slot][2 * ch + h], l);
+                        l = fmaf(s0 + s1, s.iev[slot][4 * h + g], l);
                     }
-                    tmem_store16(s_tm + 16 * ch, w);
-                    if (ch & 1) {
-                        tmem_store_wait();
-                        tcgen05_fence_before();
-                        mbar_arrive(&s.p_full[i][ch >> 1]);
-                    }
+                    tmem_store16(s_h + 16 * ch, w);
                 }
+                tmem_store_wait();
+                tcgen05_fence_before();
+                mbar_arrive(&s.p_full[i][h]);
+                o_parity ^= 1u << h;
             }
             tile_ctr += shape.most;
             if (!ok) break;
 
-            ok = __all_sync(0xffffffffu, wait_bar(&s.o_full[i], o_parity, failed));
-            if (!ok) break;
-            o_parity ^= 1u;
-            tcgen05_fence_after();
+            // epilogue
+            if (n == 0) o_parity ^= 1u;   // a segment without steps counts one, so that this row tile is never ahead of it
+            if (!(ok = wait_output(n > 0 ? (n - 1) & 1 : 0))) break;
             const int buffer = bearing & (kBadBuffers - 1);
             const bool bad = n > 0 && (volatile int &)s.bad_any[buffer] != 0;
             if (shape.most > 0) ++bearing;
@@ -628,61 +615,70 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         // ------------------------------------------------------------------ MMA issue for one row tile
         if (lane == 0) {
             const int i = warp - 9;
-            const uint32_t idesc_s = umma_idesc16(!FP8, kTileTokens, false), idesc_o = umma_idesc16(!FP8, D, true);
+            const uint32_t idesc_s = umma_idesc16(!FP8, kStepTokens, false), idesc_o = umma_idesc16(!FP8, D, true);
             const uint32_t s_tm = tmem + i * 128, o_tm = tmem + 256 + i * 128;
             uint32_t kv_it = 0, q_parity = 0, p_parity = 0;
             bool ok = true;
             const uint64_t dq = smem_desc_k_major_sw128(s.q[i]), dk0 = smem_desc_k_major_sw128(s.k[0]);
             const uint64_t dv0 = smem_desc_mn_major_sw128(s.v[0], kPanelBytes);
+            constexpr uint64_t kHalf = (uint64_t)(kStepTokens * 128 >> 4);   // 64 positions further in a key or value tile
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 ok = ok && wait_bar(bar, parity, failed);
                 return ok;
             };
-            // S = Q K^T of tile t (or, where this row tile has no use for it, only the stage's release)
-            auto scores = [&](uint32_t t, bool used) {
-                if (!wait(&s.k_full[t & 1], (t >> 1) & 1)) return;
-                if (!used) {
-                    mbar_arrive(&s.k_empty[t & 1]);
-                    return;
-                }
-                tcgen05_fence_after();
-                const uint64_t dk = dk0 + (t & 1) * (T::kOperandBytes >> 4);
+            // S = Q K^T of half h of tile t
+            auto scores = [&](uint32_t t, int h) {
+                const uint64_t dk = dk0 + (t & 1) * (T::kOperandBytes >> 4) + h * kHalf;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     const uint64_t at = (uint64_t)((ks >> 2) * (kPanelBytes >> 4) + (ks & 3) * 2);
-                    umma16_ss(s_tm, dq + at, dk + at, idesc_s, ks != 0);
+                    umma16_ss(s_tm + h * kStepTokens, dq + at, dk + at, idesc_s, ks != 0);
                 }
-                umma_commit(&s.s_full[i]);
-                umma_commit(&s.k_empty[t & 1]);
+                umma_commit(&s.s_full[i][h]);
+            };
+            // gives a stage back once this row tile's products with it are done (or at once where it has none)
+            auto release = [&](uint64_t *empty, bool used) {
+                if (used) umma_commit(empty);
+                else mbar_arrive(empty);
             };
             while (ok && advance(true)) {
                 if (!wait(&s.q_full[i], q_parity)) break;
                 q_parity ^= 1u;
                 const int n = shape.n[i];
-                if (n == 0) mbar_arrive(&s.o_full[i]);
+                if (n == 0) mbar_arrive(&s.o_done[i][0]);
                 if (shape.most == 0) continue;
-                scores(kv_it, n > 0);
+                if (!wait(&s.k_full[kv_it & 1], (kv_it >> 1) & 1)) break;
+                tcgen05_fence_after();
+                if (n > 0) scores(kv_it, 0);
+                if (n > 1) scores(kv_it, 1);
+                release(&s.k_empty[kv_it & 1], n > 0);
                 for (int j = 0; ok && j < shape.most; ++j, ++kv_it) {
                     const uint32_t stage = kv_it & 1;
                     if (!wait(&s.v_full[stage], (kv_it >> 1) & 1)) break;
-                    if (j < n) {   // a tile's weights come in halves
-                        const uint64_t dv = dv0 + stage * (T::kOperandBytes >> 4);
+                    const uint64_t dv = dv0 + stage * (T::kOperandBytes >> 4);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (!wait(&s.p_full[i][half], p_parity)) break;
+                    for (int h = 0; h < 2; ++h) {
+                        const int step = 2 * j + h;
+                        if (step < n) {
+                            if (!wait(&s.p_full[i][h], (p_parity >> h) & 1)) break;
+                            p_parity ^= 1u << h;
                             tcgen05_fence_after();
 #pragma unroll
-                            for (int ks = 4 * half; ks < 4 * half + 4; ++ks)   // 16 positions: 16 rows of 128 bytes, 8 columns of weights
-                                umma16_ts(o_tm, s_tm + 8 * ks, dv + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j | ks) != 0);
+                            for (int ks = 0; ks < kStepTokens / 16; ++ks)   // 16 positions: 16 rows of 128 bytes, 8 columns of weights
+                                umma16_ts(o_tm, s_tm + h * kStepTokens + 8 * ks, dv + h * kHalf + (uint64_t)(ks * (2048 >> 4)), idesc_o, (step | ks) != 0);
+                            umma_commit(&s.o_done[i][h]);
                         }
-                        if (!ok) break;
-                        p_parity ^= 1u;
-                        if (j + 1 == n) umma_commit(&s.o_full[i]);
-                        umma_commit(&s.v_empty[stage]);
-                    } else {
-                        mbar_arrive(&s.v_empty[stage]);
+                        if (j + 1 < shape.most) {   // the step after next takes the place of these weights
+                            if (h == 0) {
+                                if (!wait(&s.k_full[stage ^ 1], ((kv_it + 1) >> 1) & 1)) break;
+                                tcgen05_fence_after();
+                            }
+                            if (step + 2 < n) scores(kv_it + 1, h);
+                            if (h == 1) release(&s.k_empty[stage ^ 1], 2 * j + 2 < n);
+                        }
                     }
-                    if (j + 1 < shape.most) scores(kv_it + 1, j + 1 < n);
+                    if (!ok) break;
+                    release(&s.v_empty[stage], 2 * j < n);
                 }
             }
             if (*failed) {   // products in flight still write tensor memory and read shared memory
