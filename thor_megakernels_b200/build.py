@@ -1,4 +1,4 @@
-"""Builds ``libb200mk.so`` (the C-ABI CUDA library) in-tree with nvcc.
+"""Builds ``libb200mk.so`` (the C-ABI CUDA library) in-tree with nvcc, and ``_paged_binding.so`` with g++.
 
 sm_100a only; nvcc cross-compiles, so this works on a machine without a GPU.
 Run as ``python -m thor_megakernels_b200.build`` or call ``build_library()``.
@@ -13,6 +13,8 @@ from pathlib import Path
 PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 LIBRARY = PACKAGE_DIR / "libb200mk.so"
+BINDING = PACKAGE_DIR / "_paged_binding.so"
+BINDING_SOURCE = CSRC / "paged_binding.cpp"
 SOURCES = ["megakernel.cu", "nvfp4.cu", "gemv.cu", "linear_batched.cu", "batched_ops.cu", "batched_step.cu", "fp4_chain.cu",
            "paged_append.cu", "paged_attention.cu", "paged_prefill.cu", "paged.cu"]
 
@@ -74,5 +76,30 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     return LIBRARY
 
 
+def build_binding(force: bool = False) -> Path:
+    """Builds ``_paged_binding.so``, the CPython module behind ``paged`` (host code only, against the installed torch)."""
+    inputs = [BINDING_SOURCE, PACKAGE_DIR.parent / "include" / "b200_megakernel.h"]
+    if not force and BINDING.exists() and all(f.stat().st_mtime <= BINDING.stat().st_mtime for f in inputs):
+        return BINDING
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    scratch = BINDING.with_name(f"{BINDING.name}.{os.getpid()}.tmp")
+    built = subprocess.run(
+        ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+         "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"], str(BINDING_SOURCE), "-o", str(scratch),
+         f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], capture_output=True, text=True)
+    if built.returncode != 0:
+        scratch.unlink(missing_ok=True)
+        raise RuntimeError(f"g++ failed:\n{built.stdout}\n{built.stderr}")
+    os.replace(scratch, BINDING)
+    return BINDING
+
+
 if __name__ == "__main__":
     print(build_library(force=True, verbose=True))
+    print(build_binding(force=True))

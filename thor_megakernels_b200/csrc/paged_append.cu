@@ -135,7 +135,7 @@ __device__ __forceinline__ int first_slot(const Batch &bt, int first, int b) { r
 
 // D: head dimension.  ITERS: rows of one page that a thread may hold.
 template <int D, int THREADS, int ITERS, bool FP8, bool LIN>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, 768 / THREADS)   // 80 registers: 64 spill (7 prompts 74 us instead of 65), 128 leave too few threads (77)
 append_kernel(const AppendParams p) {
     pdl_wait();   // and no early start for the next kernel: see paged.cuh
     constexpr int kLanes = D / 8;                          // threads per row
