@@ -155,7 +155,7 @@ typedef struct MkStatus {
 
 /* sizeof() of the structs above as this library was compiled (0 MkModelDesc,
  * 1 MkLaunchInfo, 2 MkStatus, 3 MkNvfp4Matrix, 4 MkPagedCache, 5 MkPagedBatch,
- * 6 MkPagedAppend, 7 MkPagedAttention); lets a foreign-language binding
+ * 6 MkPagedAppend, 7 MkPagedAttention, 8 MkPagedModelCache); lets a foreign-language binding
  * verify its own struct layout.  No counterpart in the reference. */
 int mk_abi_sizeof(int32_t which);
 
@@ -580,6 +580,26 @@ typedef struct MkPagedAttention {
 } MkPagedAttention;
 int64_t mk_paged_attention_workspace(const MkPagedCache *cache, const MkPagedBatch *batch, int32_t num_q_heads);
 int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch *batch, const MkPagedAttention *args, void *stream);
+
+/*
+ * A batched handle (mk_batched_create) over a paged cache: mk_step_batched and
+ * mk_prefill_batched then append to and read `cache` instead of the descriptor's
+ * dense cache.  Layer l's pages and scales lie layer_stride elements and
+ * scale_layer_stride floats behind layer 0's.  Sequence b (slot `slot` of a prefill)
+ * owns row b of the page table; the caller puts pages there for every position before
+ * the step that reaches it.  Positions are held below min(max_pages * page_size,
+ * rope_positions); rows of a sequence without a page for them are not kept.  The
+ * table and the pages are borrowed; NULL goes back to the dense cache.  Synchronises the
+ * device and allocates the attention's workspace.
+ */
+typedef struct MkPagedModelCache {
+    MkPagedCache cache;            /* layer 0 */
+    int64_t layer_stride, scale_layer_stride;
+    const int32_t *page_table;     /* device [seqs, max_pages], rows table_stride apart */
+    int64_t table_stride;
+    int32_t seqs, max_pages;
+} MkPagedModelCache;
+int mk_batched_set_paged_cache(void *handle, const MkPagedModelCache *cache);
 
 #ifdef __cplusplus
 }

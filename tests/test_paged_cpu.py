@@ -18,7 +18,8 @@ def good():
 
 def test_struct_layouts_match():
     lib = _lib.load()
-    for which, struct in enumerate((_lib.MkPagedCache, _lib.MkPagedBatch, _lib.MkPagedAppend, _lib.MkPagedAttention), start=4):
+    for which, struct in enumerate((_lib.MkPagedCache, _lib.MkPagedBatch, _lib.MkPagedAppend, _lib.MkPagedAttention,
+                                      _lib.MkPagedModelCache), start=4):
         assert lib.mk_abi_sizeof(which) == C.sizeof(struct), struct.__name__
 
 
@@ -78,3 +79,9 @@ def test_cpu_tensors_are_refused():
         paged.attention(rows, k, k, table, one)
     with pytest.raises(ValueError):
         paged.append(rows, rows, k, k, table, one)
+
+
+def test_a_null_handle_gets_no_paged_cache():
+    lib = _lib.load()
+    assert lib.mk_batched_set_paged_cache(None, None) == _lib.MK_ERR_BAD_ARGUMENT
+    assert b"null handle" in lib.mk_last_error()

@@ -47,7 +47,7 @@ EXPORTED_SYMBOLS = [
     "mk_batched_set_activation_scale",
     "mk_fp4_chain_prepare", "mk_fp4_chain_run", "mk_fp4_chain_status", "mk_fp4_chain_destroy",
     "mk_prefill_batched", "mk_batched_set_overlap", "mk_throughput_bind", "mk_throughput_set_schedule", "mk_step_throughput",
-    "mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace",
+    "mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace", "mk_batched_set_paged_cache",
 ]
 
 
@@ -127,6 +127,13 @@ class MkPagedAttention(C.Structure):
     ]
 
 
+class MkPagedModelCache(C.Structure):
+    _fields_ = [
+        ("cache", MkPagedCache), ("layer_stride", C.c_int64), ("scale_layer_stride", C.c_int64), ("page_table", C.c_void_p),
+        ("table_stride", C.c_int64), ("seqs", C.c_int32), ("max_pages", C.c_int32),
+    ]
+
+
 class MkLaunchInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "cooperative_launch", "physical_sms", "resident_worker_capacity", "active_workers", "threads_per_cta",
@@ -200,6 +207,7 @@ def load() -> C.CDLL:
     lib.mk_paged_append.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), C.POINTER(MkPagedAppend), vp]
     lib.mk_paged_attention.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), C.POINTER(MkPagedAttention), vp]
     lib.mk_paged_attention_workspace.argtypes = [C.POINTER(MkPagedCache), C.POINTER(MkPagedBatch), i32]
+    lib.mk_batched_set_paged_cache.argtypes = [vp, C.POINTER(MkPagedModelCache)]
     lib.mk_paged_attention_workspace.restype = C.c_int64
     lib.mk_tp_init.argtypes = [vp, i32, i32, i32, vp]
     lib.mk_tp_connect.argtypes = [vp, vp, i32]

@@ -123,8 +123,12 @@ class BatchedDecoder:
     cache slot ``b``.  After ``step`` the residual stream is in ``hidden``
     ``[batch, hidden]`` and the logits in ``logits`` ``[batch, vocab]``."""
 
-    def __init__(self, model, max_batch: int, quantized: dict | None = None, activation_scale: float = 1.0):
-        """``quantized``: result of ``nvfp4.quantize_model(model)`` to run every
+    def __init__(self, model, max_batch: int, quantized: dict | None = None, activation_scale: float = 1.0, cache=None):
+        """``cache``: a ``paged.PagedKvCache`` of the model's layers and heads that ``step`` and ``prefill`` use instead of the
+        model's dense cache; sequence ``b`` is row ``b`` of its page table, and the caller reserves pages for every position
+        before the call that reaches it (``cache.reserve(b, pos + 1)``).
+
+        ``quantized``: result of ``nvfp4.quantize_model(model)`` to run every
         linear as NVFP4 x NVFP4 on the block-scaled tensor-core path (the
         activations are quantised on the fly with ``activation_scale`` as their
         tensor scale); default: bf16 weights."""
@@ -170,10 +174,22 @@ class BatchedDecoder:
         d.rope_positions = model.model.rope_cos.shape[0]
         d.hidden_states, d.logits = self.hidden.data_ptr(), self.logits.data_ptr()
         self.kv_max_len, self.kv_batch = k.shape[2], k.shape[1]
+        self.cache = cache
+        if cache is not None:
+            if cache.k.shape[0] != cfg.num_hidden_layers or cache.k.device != self.hidden.device:
+                raise ValueError("the paged cache must have the model's layers and be on its device")
+            self.kv_batch = cache.page_table.shape[0]
+            self.kv_max_len = cache.page_table.shape[1] * cache.page_size
         self.lib = _lib.load()
         self.handle = C.c_void_p()
         with torch.cuda.device(self.device):
             _lib.check(self.lib.mk_batched_create(C.byref(d), max_batch, C.byref(self.handle)))
+            if cache is not None:
+                try:
+                    _lib.check(self.lib.mk_batched_set_paged_cache(self.handle, cache.describe()))
+                except Exception:
+                    self.close()
+                    raise
             if quantized is not None:
                 _lib.check(self.lib.mk_batched_set_activation_scale(self.handle, float(activation_scale)))
 

@@ -27,6 +27,7 @@
 
 #include "../../include/b200_megakernel.h"
 #include "batched_ops.cuh"
+#include "paged.cuh"
 
 extern "C" int mk_linear_batched(const void *w_bf16, const void *x_bf16, void *y_bf16, float *partials, int32_t n, int32_t k,
                                  int32_t batch, int32_t splits, int32_t *error_word, void *stream);
@@ -88,6 +89,12 @@ struct BatchedHandle {
     bool tp_bound = false, plan_ready = false;
     int covered[256] = {};        // per layer: bit (opcode - 1) set when the schedule holds that operator
     int *covered_dev = nullptr;   // device copy, for the counter fill
+    // paged cache (mk_batched_set_paged_cache): layer 0, and where a sequence's pages are written down
+    bool paged = false;
+    MkPagedModelCache pg = {};
+    paged::Pool pool = {};
+    paged::Batch pages = {};
+    void *paged_workspace = nullptr;
     int *pos_uniform = nullptr;   // [128] positions of the rows of a pass (clamped copies of the caller's, or generated)
 };
 
@@ -252,6 +259,7 @@ struct Runner {
     int half_split;   // rotary pairing (see rope_append_kernel)
     int slice_down;   // add the down projection 2048-column slice by slice (latency interpreter) or as one addend
     int slot_fixed = -1;  // >= 0: every row reads and appends to this cache slot (rows = tokens of one prompt)
+    bool use_pages = false;  // the handle's paged cache instead of the dense one
     bo::LinOut pending;
     bool has_pending = false;
     int code = 0;
@@ -268,6 +276,27 @@ struct Runner {
         o.y = y; o.partials = splits > 1 ? partials : nullptr; o.splits = splits; o.batch = rows; o.n = n; o.scale = 1.0f;
         o.group = 0;
         return o;
+    }
+    // the rows as sequences of the paged cache: one each, or all of them new rows of slot_fixed
+    paged::Batch pages() const {
+        paged::Batch bt = h->pages;
+        bt.where = pos_ids;
+        bt.tokens = rows;
+        bt.seqs = slot_fixed >= 0 ? 1 : rows;
+        bt.per_seq = rows / bt.seqs;
+        if (slot_fixed >= 0) bt.table += slot_fixed * bt.table_stride;
+        return bt;
+    }
+    paged::Pool pool_of(int l) const {
+        paged::Pool pool = h->pool;
+        const size_t bytes = (size_t)l * h->pg.layer_stride * (pool.fp8 ? 1 : 2);
+        pool.k = (uint8_t *)pool.k + bytes;
+        pool.v = (uint8_t *)pool.v + bytes;
+        if (pool.fp8) {
+            pool.k_scales += l * h->pg.scale_layer_stride;
+            pool.v_scales += l * h->pg.scale_layer_stride;
+        }
+        return pool;
     }
     int linear(const bf16 *w, const Fp4Weight *q, const bf16 *x, bf16 *y, float *partials, int n, int k, int splits) {
         if (!h->fp4)
@@ -299,6 +328,18 @@ struct Runner {
         if (!ok(linear((const bf16 *)d.qkv_w + (size_t)l * h->qkv_rows * d.hidden_size, h->fp4 ? h->w_qkv + l : nullptr,
                        b.normed_attn, h->qkv_y, h->part_a, h->qkv_rows, d.hidden_size, h->s_qkv)))
             return;
+        if (use_pages) {
+            paged::AppendParams p = {};
+            p.bt = pages();
+            p.pool = pool_of(l);
+            p.lin = result(h->qkv_y, h->part_a, h->qkv_rows, h->s_qkv);
+            p.from_linear = true;
+            p.q_out = b.q;
+            p.hq = d.num_q_heads;
+            p.rope_cos = d.rope_cos; p.rope_sin = d.rope_sin; p.rot = d.head_dim; p.positions = d.rope_positions; p.half = half_split;
+            ok((int)paged::launch_append(p, st));
+            return;
+        }
         ok(launch_rope_append(result(h->qkv_y, h->part_a, h->qkv_rows, h->s_qkv), pos_ids, d.rope_cos, d.rope_sin, b.q, b.k_cache,
                               b.v_cache, l, rows, d.kv_batch, d.kv_max_len, d.num_q_heads, d.num_kv_heads, d.head_dim, half_split, slot_fixed, st));
     }
@@ -306,6 +347,22 @@ struct Runner {
         const MkModelDesc &d = h->d;
         flush();
         if (code) return;
+        if (use_pages) {
+            paged::AttentionParams p = {};
+            p.bt = pages();
+            p.bt.where_offset = p.bt.per_seq;   // pos_ids holds a sequence's first new position; its length ends with the last
+            const paged::Pool pool = pool_of(l);
+            p.q = b.q;
+            p.q_token = (long long)d.num_q_heads * d.head_dim;
+            p.q_head = d.head_dim;
+            p.out = b.attn;
+            p.k_scales = pool.k_scales; p.v_scales = pool.v_scales;
+            p.hq = d.num_q_heads; p.hkv = d.num_kv_heads;
+            p.group = paged::fast_div(d.num_q_heads / d.num_kv_heads);
+            p.scale_log2e = d.attn_scale * 1.4426950408889634f;
+            ok(paged::launch_attention(p, pool, h->paged_workspace, h->sms, st));
+            return;
+        }
         ok(launch_attention_batched(b.q, b.k_cache, b.v_cache, pos_ids, b.attn, h->attn_partial,
                                     attention_batched_splits(rows, d.num_kv_heads, h->sms, kMaxAttnSplits), l, rows, d.kv_batch,
                                     d.kv_max_len, d.num_q_heads, d.num_kv_heads, d.head_dim, d.attn_scale, slot_fixed, st));
@@ -369,19 +426,70 @@ struct Runner {
 }  // namespace
 }  // namespace mk
 
+// Positions a sequence can have in the handle's cache.
+static int cache_positions(const BatchedHandle *h) {
+    return h->paged ? (int)std::min((long long)h->pg.max_pages * h->pool.page_size, 0x7fffffffll) : h->d.kv_max_len;
+}
+
+extern "C" int mk_batched_set_paged_cache(void *handle, const MkPagedModelCache *c) {
+    const char *who = "mk_batched_set_paged_cache";
+    BatchedHandle *h = (BatchedHandle *)handle;
+    if (!h) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_batched_set_paged_cache: null handle");
+    const MkModelDesc &d = h->d;
+    paged::Pool pool = {};
+    paged::Batch bt = {};
+    size_t bytes = 0;
+    if (c) {
+        // the largest calls to come: a step of max_batch rows, a prompt pass of as many
+        MkPagedBatch b = {};
+        b.page_table = c->page_table; b.table_stride = c->table_stride; b.positions = h->pos_uniform; b.error_word = h->error_word;
+        b.seqs = c->seqs; b.tokens = c->seqs; b.max_pages = c->max_pages;
+        const int code = paged::read_cache(c->cache, b, MK_PAGED_MAX_SEQS, pool, bt, who);
+        if (code) return code;
+        if (pool.kv_heads != d.num_kv_heads || pool.head_dim != d.head_dim)
+            return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_batched_set_paged_cache: the cache's heads are not the model's");
+        if (c->layer_stride < 0 || c->layer_stride % (pool.fp8 ? 16 : 8) || (pool.fp8 && c->scale_layer_stride < (int64_t)pool.num_pages * pool.kv_heads) ||
+            (d.num_layers > 1 && c->layer_stride == 0))
+            return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_batched_set_paged_cache: layers overlap or do not start on 16-byte boundaries");
+        for (int whole = 0; whole < 2; ++whole) {
+            for (int rows = 1; rows <= h->max_batch; ++rows) {
+                paged::Batch call = bt;
+                call.tokens = rows;
+                call.seqs = whole ? 1 : rows;
+                call.per_seq = rows / call.seqs;
+                const long long need = paged::attention_workspace(call, pool, d.num_q_heads, h->sms);
+                if (need < 0) return fail_msg(MK_ERR_UNSUPPORTED, "mk_batched_set_paged_cache: more rows times positions than one call takes");
+                bytes = std::max(bytes, (size_t)need);
+            }
+        }
+    }
+    cudaError_t e = cudaDeviceSynchronize();   // steps on the old cache
+    if (e != cudaSuccess) return fail_msg((int)e, cudaGetErrorString(e));
+    void *workspace = nullptr;
+    if (bytes && (e = cudaMalloc(&workspace, bytes)) != cudaSuccess) return fail_msg((int)e, "mk_batched_set_paged_cache: cudaMalloc(workspace) failed");
+    if (h->paged_workspace) cudaFree(h->paged_workspace);
+    h->paged_workspace = workspace;
+    h->paged = c != nullptr;
+    h->pg = c ? *c : MkPagedModelCache{};
+    h->pool = pool;
+    h->pages = bt;
+    return 0;
+}
+
 extern "C" int mk_step_batched(void *handle, const int32_t *tokens_in, const int32_t *pos_ids, int32_t batch,
                                int32_t *tokens_out, void *stream) {
     BatchedHandle *h = (BatchedHandle *)handle;
     if (!h || !tokens_in || !pos_ids) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_step_batched: null argument");
     if (batch < 1 || batch > h->max_batch) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_step_batched: batch outside 1..max_batch");
     const MkModelDesc &d = h->d;
-    if (batch > d.kv_batch) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_step_batched: the cache holds fewer sequences than the batch");
+    if (batch > (h->paged ? h->pg.seqs : d.kv_batch)) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_step_batched: the cache holds fewer sequences than the batch");
     Runner r;
     // the kernels index with clamped copies of the caller's positions (bit 1 of the error word if any was out of range)
     r.h = h; r.st = (cudaStream_t)stream; r.pos_ids = h->pos_uniform; r.rows = batch; r.half_split = 0; r.slice_down = 1;
     r.b = StepBuffers{(bf16 *)d.hidden_states, (bf16 *)d.logits, h->normed, h->normed, h->normed, h->q, h->attn, h->act,
                       (bf16 *)d.k_cache, (bf16 *)d.v_cache};
-    r.ok(launch_sanitize_positions(pos_ids, h->pos_uniform, batch, std::min(d.kv_max_len, d.rope_positions), h->error_word, r.st));
+    r.use_pages = h->paged;
+    r.ok(launch_sanitize_positions(pos_ids, h->pos_uniform, batch, std::min(cache_positions(h), d.rope_positions), h->error_word, r.st));
     r.ok(launch_embed((const bf16 *)d.embed_w, tokens_in, r.b.hidden, batch, d.hidden_size, d.vocab_size, h->error_word, r.st));
     for (int l = 0; l < d.num_layers && r.code == 0; ++l) {
         r.attn_norm(l); r.qkv(l); r.attention(l); r.o_proj(l); r.mlp_norm(l); r.gate_up(l, true); r.down_proj(l);
@@ -402,8 +510,8 @@ extern "C" int mk_prefill_batched(void *handle, const int32_t *tokens, int32_t c
     BatchedHandle *h = (BatchedHandle *)handle;
     if (!h || !tokens) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_prefill_batched: null argument");
     const MkModelDesc &d = h->d;
-    if (count < 1 || slot < 0 || slot >= d.kv_batch || start_pos < 0 || start_pos + count > d.kv_max_len ||
-        start_pos + count > d.rope_positions)
+    if (count < 1 || slot < 0 || slot >= (h->paged ? h->pg.seqs : d.kv_batch) || start_pos < 0 ||
+        (long long)start_pos + count > cache_positions(h) || (long long)start_pos + count > d.rope_positions)
         return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_prefill_batched: prompt outside the cache / rotary tables, or slot outside the cache");
     cudaStream_t st = (cudaStream_t)stream;
     for (int c0 = 0; c0 < count; c0 += h->max_batch) {
@@ -412,6 +520,7 @@ extern "C" int mk_prefill_batched(void *handle, const int32_t *tokens, int32_t c
         if (e != cudaSuccess) return fail_msg((int)e, cudaGetErrorString(e));
         Runner r;
         r.h = h; r.st = st; r.pos_ids = h->pos_uniform; r.rows = rows; r.half_split = 0; r.slice_down = 1; r.slot_fixed = slot;
+        r.use_pages = h->paged;
         r.b = StepBuffers{(bf16 *)d.hidden_states, (bf16 *)d.logits, h->normed, h->normed, h->normed, h->q, h->attn, h->act,
                           (bf16 *)d.k_cache, (bf16 *)d.v_cache};
         r.ok(launch_embed((const bf16 *)d.embed_w, tokens + c0, r.b.hidden, rows, d.hidden_size, d.vocab_size, h->error_word, st));
@@ -588,7 +697,7 @@ extern "C" int mk_batched_status(void *handle, void *stream) {
     if (word != 0) {
         cudaMemset(h->error_word, 0, sizeof(int));
         if (word & 1) return fail_msg(MK_ERR_DEVICE_WAIT, "a bounded wait inside a batched linear ran out");
-        return fail_msg(MK_ERR_BAD_ARGUMENT, "a token id or position given to a batched step or prefill was outside the vocabulary / the cache and rotary tables; it was clamped");
+        return fail_msg(MK_ERR_BAD_ARGUMENT, "a token id or position given to a batched step or prefill was outside the vocabulary / the cache and rotary tables (it was clamped), or a page id outside the paged cache (it was left out)");
     }
     return 0;
 }
@@ -604,6 +713,7 @@ extern "C" void mk_batched_destroy(void *handle) {
     BatchedHandle *h = (BatchedHandle *)handle;
     if (!h) return;
     cudaFree(h->workspace);
+    if (h->paged_workspace) cudaFree(h->paged_workspace);
     if (h->native_scales) cudaFree(h->native_scales);
     delete[] h->w_qkv; delete[] h->w_o; delete[] h->w_up; delete[] h->w_gate; delete[] h->w_down;
     delete h;

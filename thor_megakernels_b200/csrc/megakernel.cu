@@ -1969,6 +1969,7 @@ extern "C" int mk_abi_sizeof(int32_t which) {
     case 5: return (int)sizeof(MkPagedBatch);
     case 6: return (int)sizeof(MkPagedAppend);
     case 7: return (int)sizeof(MkPagedAttention);
+    case 8: return (int)sizeof(MkPagedModelCache);
     default: return -1;
     }
 }

@@ -25,7 +25,7 @@ static int refuse(int code, const char *who, const char *text) {
 static bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 // Pool and batch of a call, or an error code.
-static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs, Pool &pool, Batch &bt, const char *who) {
+int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs, Pool &pool, Batch &bt, const char *who) {
     if (!c.k_pages || !c.v_pages || !b.page_table || !b.positions || !b.error_word)
         return refuse(MK_ERR_BAD_ARGUMENT, who, "null pointer");
     if (c.format != MK_CACHE_BF16 && c.format != MK_CACHE_E4M3) return refuse(MK_ERR_UNSUPPORTED, who, "unknown cache format");
@@ -48,7 +48,7 @@ static int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs
     pool.num_pages = c.num_pages; pool.page_size = c.page_size; pool.kv_heads = c.num_kv_heads; pool.head_dim = c.head_dim; pool.fp8 = fp8;
     bt.table = b.page_table; bt.table_stride = b.table_stride; bt.where = b.positions; bt.cu = b.cu_tokens;
     bt.seqs = b.seqs; bt.tokens = b.tokens; bt.per_seq = b.cu_tokens ? 0 : b.tokens / b.seqs;
-    bt.max_pages = b.max_pages; bt.num_pages = c.num_pages; bt.error = b.error_word;
+    bt.max_pages = b.max_pages; bt.num_pages = c.num_pages; bt.error = b.error_word; bt.where_offset = 0;
     bt.page_shift = 4;
     while ((1 << bt.page_shift) < c.page_size) ++bt.page_shift;
     return 0;

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/b200_megakernel.h"
 #include "batched_ops.cuh"
 #include "mk_device.cuh"
 
@@ -27,6 +28,7 @@ struct Batch {
     int max_pages;        // columns of the table
     int num_pages;
     int page_shift;       // log2 of the page size
+    int where_offset;     // attention: added to `where` (a caller that has the position of the last row but one keeps no second array)
     int *error;
 };
 
@@ -49,7 +51,7 @@ __device__ __forceinline__ void rows_of(const Batch &bt, int b, int &first, int 
 
 // Cached length of sequence b, held inside its page table.
 __device__ __forceinline__ int length_of(const Batch &bt, int b) {
-    const int len = __ldg(bt.where + b);
+    const int len = __ldg(bt.where + b) + bt.where_offset;
     const int held = clamp_int(len, 0, clamp_int((long long)bt.max_pages << bt.page_shift, 0, 0x7fffffff));
     if (len > held) atomicOr(bt.error, kErrorIndex);
     return held;
@@ -315,6 +317,8 @@ struct AttentionParams {
     float *partial;                     // workspace: 2 parts per CTA
     JoinEntry *entries;                 // workspace: one per CTA
 };
+// Pool and batch of a call from the public structs, or an error code (and its text) where they do not fit together.
+int read_cache(const MkPagedCache &c, const MkPagedBatch &b, int max_seqs, Pool &pool, Batch &bt, const char *who);
 // bytes of workspace; negative: more work than the kernels count
 long long attention_workspace(const Batch &bt, const Pool &pool, int hq, int sms);
 // fills the workspace pointers and max_count of p

@@ -129,3 +129,77 @@ def check_errors(device=None) -> None:
         if value & 1:
             raise _lib.MegakernelError(_lib.MK_ERR_DEVICE_WAIT, "a bounded wait inside a kernel ran out")
         raise _lib.MegakernelError(_lib.MK_ERR_BAD_ARGUMENT, "a page id, position, length or row offset given to a paged call was outside its tensor; it was left out")
+
+
+class PagedKvCache:
+    """The pages of a model and who has them.
+
+    ``k`` / ``v`` ``[layers, pages, kv_heads, page_size, head_dim]``, ``k_scales`` / ``v_scales`` ``[layers, pages, kv_heads]``
+    (8-bit only), ``page_table`` int32 ``[max_seqs, max_pages]`` on the device, -1 where a sequence has no page.  A page id stands
+    for the same place in every layer.  ``reserve`` before a call that reaches new positions, ``release`` when a sequence is done;
+    both change the table in stream order (the current stream of the device), so a step that is queued already keeps its pages'
+    ids, and a captured step sees the table as it is when it is replayed."""
+
+    def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64, max_seqs: int = 128,
+                 max_positions: int | None = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("the cache must be bf16 or float8_e4m3fn")
+        if min(num_layers, num_pages, num_kv_heads, max_seqs) < 1:
+            raise ValueError("layers, pages, heads and sequences must be positive")
+        self.page_size, self.num_pages = page_size, num_pages
+        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+        # what a page holds before its first row is never read
+        self.k, self.v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self.k_scales = self.v_scales = None
+        if dtype == torch.float8_e4m3fn:
+            self.k_scales, self.v_scales = (torch.ones(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+        columns = num_pages if max_positions is None else -(-max_positions // page_size)
+        self.page_table = torch.full((max_seqs, columns), -1, dtype=torch.int32, device=device)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._owned: list[list[int]] = [[] for _ in range(max_seqs)]
+
+    @classmethod
+    def for_model(cls, model, num_pages: int, **kwargs) -> "PagedKvCache":
+        """A cache with the layers and heads of a model container."""
+        cfg = model.config
+        return cls(cfg.num_hidden_layers, num_pages, cfg.num_key_value_heads, cfg.head_dim, device=kwargs.pop("device", model.device), **kwargs)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, seq: int, positions: int) -> None:
+        """Give sequence ``seq`` pages for positions ``0 .. positions - 1`` (those it has stay its own)."""
+        owned = self._owned[seq]
+        need = -(-positions // self.page_size)
+        if need > self.page_table.shape[1]:
+            raise ValueError(f"a sequence holds at most {self.page_table.shape[1] * self.page_size} positions, asked for {positions}")
+        if need <= len(owned):
+            return
+        if need - len(owned) > len(self._free):
+            raise MemoryError(f"{need - len(owned)} pages wanted, {len(self._free)} free")
+        new = [self._free.pop() for _ in range(need - len(owned))]
+        self.page_table[seq, len(owned):need] = torch.tensor(new, dtype=torch.int32, device=self.page_table.device)
+        owned.extend(new)
+
+    def release(self, seq: int) -> None:
+        """Take all pages of sequence ``seq`` back."""
+        self._free.extend(reversed(self._owned[seq]))
+        self._owned[seq] = []
+        self.page_table[seq].fill_(-1)
+
+    def layer(self, index: int) -> dict:
+        """One layer's tensors as keyword arguments of ``append`` and ``attention``."""
+        scales = {} if self.k_scales is None else dict(k_scales=self.k_scales[index], v_scales=self.v_scales[index])
+        return dict(k_pages=self.k[index], v_pages=self.v[index], page_table=self.page_table, **scales)
+
+    def describe(self) -> _lib.MkPagedModelCache:
+        """The cache as ``mk_batched_set_paged_cache`` takes it."""
+        layers, pages, heads, size, dim = self.k.shape
+        scales = (None, None) if self.k_scales is None else (self.k_scales.data_ptr(), self.v_scales.data_ptr())
+        first = _lib.MkPagedCache(self.k.data_ptr(), self.v.data_ptr(), *scales, heads * size * dim, size * dim, dim,
+                                  _lib.MK_CACHE_BF16 if self.k_scales is None else _lib.MK_CACHE_E4M3, pages, size, heads, dim, 0)
+        return _lib.MkPagedModelCache(first, pages * heads * size * dim, pages * heads, self.page_table.data_ptr(), self.page_table.shape[1],
+                                      self.page_table.shape[0], self.page_table.shape[1])
