@@ -729,12 +729,14 @@ join_kernel(const AttentionParams p, int rows_per_block) {
 // host side
 // ---------------------------------------------------------------------------
 
-// Query rows that a sequence of this call can have at most, in tiles of 8, rounded up to 1, 2 or 4
-// tiles per row block (a block of more rows reads the cache once for all of them).
+// Tiles of 8 query rows per row block: one where no sequence of this call can have more rows, else two.  Four
+// would read the cache once for 17 to 32 rows, but their accumulators leave too few registers: 32 sequences x 5
+// tokens x 4 heads of a group against up to 16384 positions of E4M3, D = 128: one tile 256 us, two 187, four 294;
+// 16 x 5 x 4 against 4000 of bf16: 122, 86 and 108.  (12 rows: one tile 43.4, two 36.8.)
 static int row_tiles(const Batch &bt, int group, int max_count) {
     const long long most = bt.cu ? (bt.tokens < max_count ? bt.tokens : max_count) : bt.per_seq;
     const long long rows = most * group;
-    return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    return rows <= 8 ? 1 : 2;
 }
 
 bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens, bool swizzle) {
@@ -774,11 +776,8 @@ static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, 
 
 template <int D, bool FP8>
 static int launch_decode_d(const AttentionParams &p, const Pool &pool, int sms, cudaStream_t st) {
-    switch (row_tiles(p.bt, p.group.d, p.max_count)) {
-    case 1: return launch_decode_t<D, FP8, 1>(p, pool, sms, st);
-    case 2: return launch_decode_t<D, FP8, 2>(p, pool, sms, st);
-    default: return launch_decode_t<D, FP8, 4>(p, pool, sms, st);
-    }
+    if (row_tiles(p.bt, p.group.d, p.max_count) == 1) return launch_decode_t<D, FP8, 1>(p, pool, sms, st);
+    return launch_decode_t<D, FP8, 2>(p, pool, sms, st);
 }
 
 DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count, int sms) {
@@ -806,8 +805,10 @@ int launch_decode(const AttentionParams &p, const Pool &pool, int sms, cudaStrea
     return pool.fp8 ? launch_decode_d<128, true>(p, pool, sms, st) : launch_decode_d<128, false>(p, pool, sms, st);
 }
 
-// Most new tokens of a sequence that the few-row kernel takes: those whose rows fit one row block of
-// 32, so that it reads the cache once.  More rows are work for the tensor cores' large tiles.
+// Most new tokens of a sequence that the few-row kernel takes: 32 rows, two row blocks (the second finds the
+// cache's tiles in L2).  More are work for the large tiles of tcgen05, which always compute 256 rows: 20 rows
+// against up to 16384 positions of E4M3 187 us here, 259 there; with bf16 (16 x 4000) 86 and 62, but there a
+// weight is one bf16 term, here two, and a draft's tokens should meet the sums that single tokens meet.
 static int most_few(int group) { return group >= 32 ? 1 : 32 / group; }
 
 struct Plan {
