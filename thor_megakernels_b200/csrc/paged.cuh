@@ -299,7 +299,8 @@ struct AppendParams {
     int rot, positions, half;
     Pool pool;
     int hq;
-    int slots;                          // page slots per sequence (without cu)
+    FastDiv slots, per_seq;             // page slots and tokens per sequence (without cu)
+    FastDiv kv_heads, q_groups;         // groups of query heads per token
     int kv_blocks;                      // CTAs that store keys and values; the rest rotate queries
 };
 cudaError_t launch_append(AppendParams p, cudaStream_t st);

@@ -13,11 +13,16 @@
 // their codes are multiplied by a power of two, which is exact down to E4M3's subnormals.  A
 // scale only grows while its page holds rows; the first row of a page starts afresh.
 //
-// Work split.  One CTA owns the rows that a call adds to one (page, KV head): its first half
-// takes keys, its second values, 16 bytes of bf16 per thread and row, every row in registers
-// between the magnitude's reduction and the store, so that each input is read once.  Pages of
-// one sequence belong to nobody else, hence no atomics.  Query rows need no such grouping:
-// a thread keeps the table's elements of its 8 columns and walks over heads of one token.
+// Work split.  One CTA owns the keys or the values that a call adds to one (page, KV head), 16 bytes of
+// bf16 per thread and row; every row stays in registers between the magnitude's reduction and the store, so
+// that each input is read once.  Pages of one sequence belong to nobody else, hence no atomics.  Query rows
+// need no such grouping: a thread keeps the table's elements of its 8 columns for a few heads of one token.
+//
+// What bounds it.  Prompts (7 of 601 to 2100 rows, 32 query and 8 KV heads, D = 128, E4M3): 47 us on the device,
+// 4.8 TB/s.  The query rows alone run at the copy bandwidth; keys and values take half of the time for a
+// quarter of the bytes, waiting for one load after the other (sequence, start, page, tables).  With products and
+// sums one at a time and 64-bit divisions the instructions bounded it: 54 us, 75 % of the issue slots.
+// A few rows: one launch, 2.3 to 3.5 us (128 sequences x 1 row 3.4 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -30,7 +35,7 @@
 namespace mk {
 namespace paged {
 
-constexpr int kQueryHeads = 8;        // query heads of one token that a thread rotates with the same table elements
+constexpr int kQueryHeads = 4;        // query heads of one token that a thread rotates with the same table elements (8: no faster)
 constexpr int kScaleMin = -64, kScaleMax = 120;
 
 __device__ __forceinline__ uint4 pack_bf16(const float (&x)[8]) {
@@ -56,52 +61,96 @@ __device__ __forceinline__ uint4 load8(const AppendParams &p, const Rows &r, int
     }
 }
 
-__device__ __forceinline__ void load_table(const float *table, long long at, float (&x)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(table + at)), b = __ldg(reinterpret_cast<const float4 *>(table + at) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// Two products or sums at once, each rounded by itself.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 
-// Rotates the 8 elements at column 8 * chunk.  `lane_chunk0`: lane of the row's first chunk.  All lanes of a warp call it.
-__device__ __forceinline__ void rotate8(float (&x)[8], const float (&c)[8], const float (&s)[8], int chunk, int lane_chunk0, int rot,
-                                        int half) {
-    const bool inside = 8 * chunk < rot;
-    if (half) {
-        const int away = rot / 16;   // chunks between the two elements of a pair
-        const bool second = chunk >= away;
-        const int partner = lane_chunk0 + (inside ? (second ? chunk - away : chunk + away) : chunk);
+// What a thread needs to rotate the 8 elements at its column: where their pairs are, and the sign of the pair's sine.
+struct Turn {
+    bool inside, half;   // half: pairs lie rot / 2 apart, in the lane `partner`; else side by side
+    int partner;
+    float2 sign;
+};
+
+__device__ __forceinline__ Turn turn_of(int chunk, int lane_chunk0, int rot, bool half) {
+    Turn u;
+    u.inside = 8 * chunk < rot;
+    u.half = half;
+    const int away = rot / 16;   // chunks between the two elements of a pair
+    const bool second = chunk >= away;
+    u.partner = lane_chunk0 + (u.inside ? (second ? chunk - away : chunk + away) : chunk);
+    const float first = half && second ? 1.f : -1.f;
+    u.sign = make_float2(first, half ? first : 1.f);
+    return u;
+}
+
+// Cosines and signed sines of one position at 8 columns.
+struct Angles {
+    float2 c[4], s[4];
+};
+__device__ __forceinline__ void load_angles(const float *cosines, const float *sines, long long at, const Turn &u, Angles &g) {
+    const float4 c0 = __ldg(reinterpret_cast<const float4 *>(cosines + at)), c1 = __ldg(reinterpret_cast<const float4 *>(cosines + at) + 1);
+    const float4 s0 = __ldg(reinterpret_cast<const float4 *>(sines + at)), s1 = __ldg(reinterpret_cast<const float4 *>(sines + at) + 1);
+    g.c[0] = make_float2(c0.x, c0.y); g.c[1] = make_float2(c0.z, c0.w);
+    g.c[2] = make_float2(c1.x, c1.y); g.c[3] = make_float2(c1.z, c1.w);
+    g.s[0] = mul2(make_float2(s0.x, s0.y), u.sign); g.s[1] = mul2(make_float2(s0.z, s0.w), u.sign);
+    g.s[2] = mul2(make_float2(s1.x, s1.y), u.sign); g.s[3] = mul2(make_float2(s1.z, s1.w), u.sign);
+}
+
+__device__ __forceinline__ void widen(uint32_t w, float2 &x) { x = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+// 8 bf16 elements, rotated, in fp32: x c + pair(x) (+-s), both products rounded.  All lanes of a warp call it.
+__device__ __forceinline__ void rotate8(const uint4 &raw, const Angles &g, const Turn &u, float2 (&x)[4]) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w}, o[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_sync(0xffffffffu, x[i], partner);
-            if (inside) x[i] = __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(second ? other : -other, s[i]));
-        }
-    } else if (inside) {
+    for (int i = 0; i < 4; ++i) {
+        o[i] = u.half ? __shfl_sync(0xffffffffu, w[i], u.partner) : __byte_perm(w[i], 0, 0x1032);
+        widen(w[i], x[i]);
+    }
+    if (u.inside) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const float a = x[i], b = x[i + 1];
-            x[i] = __fadd_rn(__fmul_rn(a, c[i]), __fmul_rn(-b, s[i]));
-            x[i + 1] = __fadd_rn(__fmul_rn(b, c[i + 1]), __fmul_rn(a, s[i + 1]));
+        for (int i = 0; i < 4; ++i) {
+            float2 y;
+            widen(o[i], y);
+            x[i] = add2(mul2(x[i], g.c[i]), mul2(y, g.s[i]));
         }
     }
 }
 
-__device__ __forceinline__ uint2 pack_e4m3(const float (&x)[8], float factor) {
+__device__ __forceinline__ uint4 round8(const float2 (&x)[4]) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * factor, x[2 * i + 1] * factor), __NV_SATFINITE, __NV_E4M3);
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[i].x, x[i].y);
+        w[i] = *reinterpret_cast<const uint32_t *>(&v);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint2 pack_e4m3(const float2 (&x)[4], float factor) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(mul2(x[i], make_float2(factor, factor)), __NV_SATFINITE, __NV_E4M3);
     return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
 __device__ __forceinline__ uint2 recode_e4m3(uint2 codes, float factor) {
-    float x[8];
+    float2 x[4];
     const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i % 2))), __NV_E4M3);
-        const float2 f = __half22float2(__half2(h));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        x[i] = __half22float2(__half2(h));
     }
     return pack_e4m3(x, factor);
 }
@@ -133,34 +182,26 @@ __device__ __forceinline__ int find_sequence(const Batch &bt, int x, Key key) {
 // are enough for every page its rows can touch, wherever in a page they start.
 __device__ __forceinline__ int first_slot(const Batch &bt, int first, int b) { return (first >> bt.page_shift) + 2 * b; }
 
-// D: head dimension.  ITERS: rows of one page that a thread may hold.
-template <int D, int THREADS, int ITERS, bool FP8, bool LIN>
-__global__ void __launch_bounds__(THREADS, 768 / THREADS)   // 80 registers: 64 spill (7 prompts 74 us instead of 65), 128 leave too few threads (77)
+// D: head dimension.  ITERS: rows of one page that a thread may hold.  BOTH: half of a CTA takes a page's keys, half its
+// values; else they are two CTAs.
+template <int D, int THREADS, int ITERS, bool BOTH, bool FP8, bool LIN>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)   // 64 registers; 7 prompts: 80 54 us, 40 60 us (spills)
 append_kernel(const AppendParams p) {
     pdl_wait();   // and no early start for the next kernel: see paged.cuh
     constexpr int kLanes = D / 8;                          // threads per row
-    constexpr int kHalf = THREADS / 2, kHalfWarps = kHalf / 32;
-    constexpr int kRows = kHalf / kLanes;                  // rows per pass of half a CTA
-    __shared__ float amax_s[2 * kHalfWarps];
+    constexpr int kPart = BOTH ? THREADS / 2 : THREADS, kPartWarps = kPart / 32;
+    constexpr int kRows = kPart / kLanes;                  // rows per pass
+    __shared__ float amax_s[THREADS / 32];
     const Batch &bt = p.bt;
     const int lane = threadIdx.x & 31, chunk = threadIdx.x % kLanes, lane0 = lane - chunk;
     const bool rope = p.rope_cos != nullptr;
-    // table elements of a position for this thread's columns
-    auto tables = [&](long long want, bool live, float (&c)[8], float (&s)[8]) {
-        const int pos = clamp_int(want, 0, p.positions - 1);
-        if (live && pos != want) atomicOr(bt.error, kErrorIndex);
-        if (8 * chunk < p.rot) {
-            load_table(p.rope_cos, (long long)pos * p.rot + 8 * chunk, c);
-            load_table(p.rope_sin, (long long)pos * p.rot + 8 * chunk, s);
-        }
-    };
+    const Turn turn = turn_of(chunk, lane0, p.rot, p.half);
 
     if ((int)blockIdx.x >= p.kv_blocks) {                  // query rows: one token, kQueryHeads heads per thread
         constexpr int kUnits = THREADS / kLanes;           // (token, group of heads) pairs per CTA
-        const int groups = (p.hq + kQueryHeads - 1) / kQueryHeads;
-        const long long unit0 = (long long)((int)blockIdx.x - p.kv_blocks) * kUnits, unit = unit0 + threadIdx.x / kLanes;
-        int t = (int)(unit / groups);
-        const int head0 = (int)(unit % groups) * kQueryHeads;
+        const int unit = ((int)blockIdx.x - p.kv_blocks) * kUnits + (int)threadIdx.x / kLanes;
+        int t = div(unit, p.q_groups);
+        const int head0 = (unit - t * p.q_groups.d) * kQueryHeads;
         bool live = t < bt.tokens;
         t = min(t, bt.tokens - 1);
         uint4 raw[kQueryHeads];
@@ -168,40 +209,49 @@ append_kernel(const AppendParams p) {
         for (int i = 0; i < kQueryHeads; ++i) raw[i] = head0 + i < p.hq ? load8<LIN>(p, p.q, 0, t, head0 + i, 8 * chunk) : make_uint4(0u, 0u, 0u, 0u);
         int b;
         if (bt.cu) {
-            b = find_sequence(bt, (int)(unit0 / groups), [](int first, int) { return first; });
+            b = find_sequence(bt, __shfl_sync(0xffffffffu, t, 0), [](int first, int) { return first; });
             while (b + 1 < bt.seqs && __ldg(bt.cu + b + 1) <= t) ++b;
         } else {
-            b = t / bt.per_seq;
+            b = div(t, p.per_seq);
         }
         int first, count;
         rows_of(bt, b, first, count);
         const int start = __ldg(bt.where + b);
         live = live && start >= 0 && t >= first && t < first + count;   // idle sequences' rows stay as they were
-        float c[8] = {}, s[8] = {};
-        if (rope) tables((long long)start + (t - first), live, c, s);
+        Angles angles;
+        if (rope) {
+            const long long want = (long long)start + (t - first);
+            const int pos = clamp_int(want, 0, p.positions - 1);
+            if (live && pos != want) atomicOr(bt.error, kErrorIndex);
+            if (turn.inside) load_angles(p.rope_cos, p.rope_sin, (long long)pos * p.rot + 8 * chunk, turn, angles);
+        }
+        bf16 *dst = p.q_out + ((long long)t * p.hq + head0) * D + 8 * chunk;
 #pragma unroll
         for (int i = 0; i < kQueryHeads; ++i) {
-            float x[8];
-            unpack8(raw[i], x);
-            if (rope) rotate8(x, c, s, chunk, lane0, p.rot, p.half);
-            if (live && head0 + i < p.hq)
-                *reinterpret_cast<uint4 *>(p.q_out + ((long long)t * p.hq + head0 + i) * D + 8 * chunk) = pack_bf16(x);
+            uint4 out = raw[i];
+            if (rope) {
+                float2 x[4];
+                rotate8(raw[i], angles, turn, x);
+                out = round8(x);
+            }
+            if (live && head0 + i < p.hq) *reinterpret_cast<uint4 *>(dst + i * D) = out;
         }
         return;
     }
 
     // keys and values of one (page, KV head)
     const int hkv = p.pool.kv_heads, page_size = 1 << bt.page_shift;
-    const int slot = blockIdx.x / hkv, head = blockIdx.x % hkv;
-    const bool is_v = threadIdx.x >= kHalf;
-    const int row_in_pass = (threadIdx.x % kHalf) / kLanes;
+    const int pair = BOTH ? blockIdx.x : blockIdx.x >> 1;
+    const int slot = div(pair, p.kv_heads), head = pair - slot * hkv;
+    const bool is_v = BOTH ? threadIdx.x >= kPart : blockIdx.x & 1;
+    const int row_in_pass = (threadIdx.x % kPart) / kLanes;
     int b, ordinal;
     if (bt.cu) {
         b = find_sequence(bt, slot, [&](int first, int at) { return first_slot(bt, first, at); });
         ordinal = slot - first_slot(bt, clamp_int(__ldg(bt.cu + b), 0, bt.tokens), b);
     } else {
-        b = slot / p.slots;
-        ordinal = slot % p.slots;
+        b = div(slot, p.slots);
+        ordinal = slot - b * p.slots.d;
     }
     int first, count;
     rows_of(bt, b, first, count);
@@ -233,13 +283,18 @@ append_kernel(const AppendParams p) {
         if (threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
         return;
     }
+    const bool rotated = rope && !is_v;
+    if (rotated && page_begin + end > p.positions && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
+    const long long pos0 = page_begin + held;
     // row `it` of this thread in fp32, keys rotated
-    auto value = [&](int it, float (&x)[8]) {
-        unpack8(raw[it], x);
-        if (rope && !is_v) {
-            float c[8] = {}, s[8] = {};
-            tables(page_begin + held + min(it * kRows + row_in_pass, added - 1), true, c, s);
-            rotate8(x, c, s, chunk, lane0, p.rot, p.half);
+    auto value = [&](int it, float2 (&x)[4]) {
+        if (rotated) {
+            const int pos = clamp_int(pos0 + min(it * kRows + row_in_pass, added - 1), 0, p.positions - 1);
+            Angles angles;
+            if (turn.inside) load_angles(p.rope_cos, p.rope_sin, (long long)pos * p.rot + 8 * chunk, turn, angles);
+            rotate8(raw[it], angles, turn, x);
+        } else {
+            widen(raw[it].x, x[0]); widen(raw[it].y, x[1]); widen(raw[it].z, x[2]); widen(raw[it].w, x[3]);
         }
     };
     const long long base = page * p.pool.page_stride + head * p.pool.head_stride + 8 * chunk;
@@ -249,28 +304,33 @@ append_kernel(const AppendParams p) {
         for (int it = 0; it < ITERS; ++it) {
             if (it * kRows < added) {
                 const int i = it * kRows + row_in_pass;
-                float x[8];
+                float2 x[4];
                 value(it, x);
-                if (i < added) *reinterpret_cast<uint4 *>(dst + (held + i) * p.pool.slot_stride) = pack_bf16(x);
+                if (i < added) *reinterpret_cast<uint4 *>(dst + (held + i) * p.pool.slot_stride) = round8(x);
             }
         }
     } else {
-        // The rotation is done twice, for the magnitude and for the store, where a thread holds many rows: their fp32
-        // values would cost twice the registers, and the tables' elements are in L1 by then.
-        constexpr bool kKeep = ITERS <= 2;
-        float kept[kKeep ? ITERS : 1][8];
-        float amax = 0.f;
+        float2 kept[ITERS][4];
+        float amax = 0.f;                                      // NaN never enters
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
             if (it * kRows < added) {
-                float (&x)[8] = kept[kKeep ? it : 0];
-                value(it, x);
+                value(it, kept[it]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float a = fabsf(x[j]);
-                    if (a < INFINITY) amax = fmaxf(amax, a);
-                }
+                for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(kept[it][j].x), fabsf(kept[it][j].y)));
             }
+        }
+        if (amax == INFINITY) {                                // infinities saturate: the finite elements set the scale
+            amax = 0.f;
+            auto finite = [&](float a) { if (a < INFINITY) amax = fmaxf(amax, a); };
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it)
+                if (it * kRows < added)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        finite(fabsf(kept[it][j].x));
+                        finite(fabsf(kept[it][j].y));
+                    }
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
@@ -280,7 +340,7 @@ append_kernel(const AppendParams p) {
         __syncthreads();                                       // after every thread's read of the scale, too
         amax = 0.f;
 #pragma unroll
-        for (int w = 0; w < kHalfWarps; ++w) amax = fmaxf(amax, amax_s[(is_v ? kHalfWarps : 0) + w]);
+        for (int w = 0; w < kPartWarps; ++w) amax = fmaxf(amax, amax_s[(BOTH && is_v ? kPartWarps : 0) + w]);
         const float need = __uint_as_float((uint32_t)(scale_exponent(amax) + 127) << 23);
         const float scale = fmaxf(old, need);
         uint8_t *dst = reinterpret_cast<uint8_t *>(is_v ? p.pool.v : p.pool.k) + base;
@@ -292,27 +352,30 @@ append_kernel(const AppendParams p) {
                 *at = recode_e4m3(*at, factor);
             }
         }
-        if (threadIdx.x % kHalf == 0) *scales = scale;
+        if (threadIdx.x % kPart == 0) *scales = scale;
         const float inverse = 1.0f / scale;                    // exact: a power of two
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
             if (it * kRows < added) {
                 const int i = it * kRows + row_in_pass;
-                float (&x)[8] = kept[kKeep ? it : 0];
-                if constexpr (!kKeep) value(it, x);
-                if (i < added) *reinterpret_cast<uint2 *>(dst + (held + i) * p.pool.slot_stride) = pack_e4m3(x, inverse);
+                if (i < added) *reinterpret_cast<uint2 *>(dst + (held + i) * p.pool.slot_stride) = pack_e4m3(kept[it], inverse);
             }
         }
     }
 }
 
-template <int D, int THREADS, int ITERS, bool FP8, bool LIN>
+template <int D, int THREADS, int ITERS, bool BOTH, bool FP8, bool LIN>
 static cudaError_t launch_append_t(AppendParams &p, long long kv, cudaStream_t st) {
     const int groups = (p.hq + kQueryHeads - 1) / kQueryHeads, per_cta = THREADS * 8 / D;
-    const long long q = p.q_out ? ((long long)p.bt.tokens * groups + per_cta - 1) / per_cta : 0;
+    const long long units = p.q_out ? (long long)p.bt.tokens * groups : 0, q = (units + per_cta - 1) / per_cta;
+    if (units + per_cta > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    p.q_groups = fast_div(groups ? groups : 1);
+    p.kv_heads = fast_div(p.pool.kv_heads);
+    p.per_seq = fast_div(p.bt.cu ? 1 : p.bt.per_seq);
+    if (!BOTH) kv *= 2;
     if (kv + q > 0x7fffffff) return cudaErrorInvalidConfiguration;
     p.kv_blocks = (int)kv;
-    return launch_pdl(append_kernel<D, THREADS, ITERS, FP8, LIN>, dim3((unsigned)(kv + q)), dim3(THREADS), 0, st, p);
+    return launch_pdl(append_kernel<D, THREADS, ITERS, BOTH, FP8, LIN>, dim3((unsigned)(kv + q)), dim3(THREADS), 0, st, p);
 }
 
 template <int D, bool FP8, bool LIN>
@@ -320,14 +383,14 @@ static cudaError_t launch_append_d(AppendParams &p, long long kv, int rows, cuda
     // A few rows per page (decoding): a warp each for keys and values, so that every CTA of a large batch is resident at
     // once (128 sequences x 8 heads: 12.7 us with the wide CTAs below, 4 with these).
     constexpr int kFew = 32 * 8 / D;   // rows of one pass of a warp
-    if (rows <= kFew) return launch_append_t<D, 64, 1, FP8, LIN>(p, kv, st);
-    if (rows <= 2 * kFew) return launch_append_t<D, 64, 2, FP8, LIN>(p, kv, st);
+    if (rows <= kFew) return launch_append_t<D, 64, 1, true, FP8, LIN>(p, kv, st);
+    if (rows <= 2 * kFew) return launch_append_t<D, 64, 2, true, FP8, LIN>(p, kv, st);
     switch (p.pool.page_size * D / 1024) {
-    case 1: return launch_append_t<D, 256, 1, FP8, LIN>(p, kv, st);
-    case 2: return launch_append_t<D, 256, 2, FP8, LIN>(p, kv, st);
-    case 4: return launch_append_t<D, 256, 4, FP8, LIN>(p, kv, st);
-    case 8: return launch_append_t<D, 256, 8, FP8, LIN>(p, kv, st);
-    case 16: return launch_append_t<D, 256, 16, FP8, LIN>(p, kv, st);
+    case 1: return launch_append_t<D, 128, 1, false, FP8, LIN>(p, kv, st);
+    case 2: return launch_append_t<D, 256, 1, false, FP8, LIN>(p, kv, st);
+    case 4: return launch_append_t<D, 256, 2, false, FP8, LIN>(p, kv, st);
+    case 8: return launch_append_t<D, 256, 4, false, FP8, LIN>(p, kv, st);
+    case 16: return launch_append_t<D, 512, 4, false, FP8, LIN>(p, kv, st);
     default: return cudaErrorInvalidValue;
     }
 }
@@ -339,10 +402,10 @@ static cudaError_t launch_append_l(AppendParams &p, cudaStream_t st) {
     long long slots;
     if (bt.cu) {
         slots = bt.tokens / page + 2ll * bt.seqs;
-        p.slots = 0;
+        p.slots = fast_div(1);
     } else {
-        p.slots = bt.per_seq == 1 ? 1 : (bt.per_seq - 1) / page + 2;
-        slots = (long long)p.slots * bt.seqs;
+        p.slots = fast_div(bt.per_seq == 1 ? 1 : (bt.per_seq - 1) / page + 2);
+        slots = (long long)p.slots.d * bt.seqs;
     }
     const long long kv = slots * p.pool.kv_heads;
     const int rows = most < page ? most : page;
