@@ -571,7 +571,7 @@ int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *batch, const 
  */
 typedef struct MkPagedAttention {
     const void *q;
-    void *out;                     /* bf16 [tokens, num_q_heads, head_dim] */
+    void *out;                     /* bf16 [tokens, num_q_heads, head_dim], not overlapping q */
     void *workspace;
     int64_t workspace_bytes;
     int64_t q_token_stride, q_head_stride;
@@ -590,7 +590,7 @@ int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch *batch, con
  * the step that reaches it.  Positions are held below min(max_pages * page_size,
  * rope_positions); rows of a sequence without a page for them are not kept.  The
  * table and the pages are borrowed; NULL goes back to the dense cache.  Synchronises the
- * device and allocates the attention's workspace.
+ * device and allocates the attention's workspace anew: CUDA graphs of earlier steps are void.
  */
 typedef struct MkPagedModelCache {
     MkPagedCache cache;            /* layer 0 */

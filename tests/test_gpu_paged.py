@@ -636,3 +636,127 @@ def test_refusals_on_the_device():
     refused(paged.append, odd, rows, k, v, table, one)                         # not on a 16-byte boundary
     assert paged.attention(q[:0], k, v, table[:0], one[:0], cu_tokens=ints([0])).shape == (0, 4, 64)
     paged.check_errors()
+
+
+# --------------------------------------------------------------------------- calls that are easy to forget
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[1, 3], [70, 9]])
+@pytest.mark.parametrize("scale", [-0.7, 0.0])
+def test_negative_and_zero_scales(dtype, new, scale):
+    run_attention(dtype, 64, 16, 4, 1, new, [150, 300], seed=41, scale=scale, q_size=3.0)
+
+
+@pytest.mark.parametrize("layout,rot", [("interleaved", 64), ("half", 32)])
+def test_rotation_in_place(layout, rot):
+    from thor_megakernels_b200 import paged
+
+    gen = generator(42)
+    k, v, _, _ = pool(torch.bfloat16, 8, 2, 16, 64, gen)
+    rows = torch.randn((37, 2, 64), generator=gen, device="cuda").bfloat16()
+    q = torch.randn((37, 9, 64), generator=gen, device="cuda").bfloat16()
+    angle = torch.rand((64, rot), generator=gen, device="cuda") * 6
+    args = (rows, rows, k, v, torch.arange(3, device="cuda").int().view(1, 3), ints([5]))
+    tables = dict(rope_cos=angle.cos(), rope_sin=angle.sin(), layout=layout)
+    want = paged.append(*args, q=q, **tables)
+    got = paged.append(*args, q=q, q_out=q, **tables)
+    assert got is q and torch.equal(got, want)
+    paged.check_errors()
+
+
+def test_overlapping_outputs_are_refused():
+    from thor_megakernels_b200 import paged
+
+    k, v, _, _ = pool(torch.bfloat16, 4, 2, 16, 64, generator(43))
+    buffer = torch.zeros((6, 4, 64), dtype=torch.bfloat16, device="cuda")
+    q, table, start = buffer[:4], ints([[0, 1]]), ints([0])
+    rows = buffer.view(12, 2, 64)[:4]
+    other = torch.zeros((4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        paged.attention(q, k, v, table, ints([4]), out=q)
+    with pytest.raises(ValueError, match="overlap"):
+        paged.attention(q, k, v, table, ints([4]), out=buffer[2:])
+    with pytest.raises(ValueError, match="overlap"):
+        paged.append(other, other, k, v, table, start, q=q, q_out=buffer[2:])
+    with pytest.raises(ValueError, match="overlap"):
+        paged.append(rows, other, k, v, table, start, q=torch.zeros_like(q), q_out=q)
+    packed = torch.zeros((1, 8, 64), dtype=torch.bfloat16, device="cuda")   # side by side is not overlapping
+    paged.append(packed[:, 4:6], packed[:, 6:], k, v, table, start, q=packed[:, :4], q_out=packed[:, :4])
+    paged.check_errors()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_that_do_not_grow_are_reported(dtype):
+    """Rows and pages of no sequence stay as they were, and the next call is right."""
+    from thor_megakernels_b200 import paged
+    from thor_megakernels_b200._lib import MegakernelError
+
+    gen = generator(44)
+    k, v, ks, vs = pool(dtype, 40, 2, 16, 64, gen)
+    rows = torch.randn((64, 2, 64), generator=gen, device="cuda").bfloat16()
+    q = torch.randn((64, 8, 64), generator=gen, device="cuda").bfloat16()
+    table = torch.arange(30, device="cuda").int().view(5, 6)
+    scales = dict(k_scales=ks, v_scales=vs)
+    for cu in ([0, 50, 20, 64, 3, 64], [60, 40, 20, 10, 5, 0], [-5, 70, 2 ** 31 - 1, -2 ** 31, 8, 64], [64, 0, 64, 0, 64, 0]):
+        kept = [t[30:].clone() for t in (k, v)]
+        paged.append(rows, rows, k, v, table, ints([3, 0, 17, 20, 1]), q=q, cu_tokens=ints(cu), **scales)
+        with pytest.raises(MegakernelError):
+            paged.check_errors()
+        for a, b in zip((k, v), kept):
+            assert torch.equal(a[30:].view(torch.uint8), b.view(torch.uint8))
+        out = paged.attention(q, k, v, table, ints([80, 96, 60, 90, 70]), cu_tokens=ints(cu), **scales)
+        assert out.shape == q.shape
+        with pytest.raises(MegakernelError):
+            paged.check_errors()
+    run_attention(dtype, 64, 16, 8, 2, [40, 24], [80, 96], seed=45)
+
+
+def test_offsets_that_repeat_all_rows_for_many_sequences():
+    """512 sequences claim the same 4096 rows over a million positions each: more work than an int counts.  Nothing is done.
+    (256 row blocks x 4 KV heads x at least 8160 tiles x 512 = 4.3e9; with a group of 8 heads it would be 2.144e9, just below.)"""
+    from thor_megakernels_b200 import paged
+    from thor_megakernels_b200._lib import MegakernelError
+
+    k, v, _, _ = pool(torch.bfloat16, 2, 4, 128, 64, generator(46))
+    q = torch.ones((4096, 64, 64), dtype=torch.bfloat16, device="cuda")
+    table = torch.full((1024, 8192), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.full((1024,), 1 << 20, dtype=torch.int32, device="cuda")
+    cu = ints([0, 4096] * 512 + [0])
+    out = torch.full_like(q, 7.0)
+    paged.attention(q, k, v, table, lengths, cu_tokens=cu, out=out)
+    with pytest.raises(MegakernelError):
+        paged.check_errors()
+    assert (out == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_captured_append_and_attention_follow_their_inputs(dtype):
+    from thor_megakernels_b200 import paged
+
+    gen = generator(47)
+    pools = [pool(dtype, 40, 2, 32, 64, generator(48)) for _ in range(2)]   # alike
+    table = torch.randperm(40, generator=gen, device="cuda").int().view(4, 10)
+    steps = [(ints(s), [torch.randn((4 * n, h, 64), generator=gen, device="cuda").bfloat16() for h in (8, 2, 2)])
+             for n, s in ((3, [0, 5, 100, 250]), (3, [3, 8, 103, 253]), (3, [6, 11, -1, 256]))]
+    angle = torch.rand((320, 64), generator=gen, device="cuda") * 6
+    cos, sin = angle.cos(), angle.sin()
+
+    def step(p, start, q, k, v):
+        scales = dict(k_scales=p[2], v_scales=p[3])
+        rotated = paged.append(k, v, p[0], p[1], table, start, q=q, rope_cos=cos, rope_sin=sin, q_out=torch.zeros_like(q), **scales)
+        return paged.attention(rotated, p[0], p[1], table, torch.where(start < 0, 0, start + 3).int(), **scales)
+
+    want = [step(pools[0], start, *rows) for start, rows in steps]
+    start, rows = steps[0][0].clone(), [t.clone() for t in steps[0][1]]
+    start.fill_(-1)
+    step(pools[1], start, *rows)   # idle: stores nothing
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(pools[1], start, *rows)
+    for (s, r), w in zip(steps, want):
+        start.copy_(s)
+        for a, b in zip(rows, r):
+            a.copy_(b)
+        graph.replay()
+        assert torch.equal(got, w)
+    paged.check_errors()

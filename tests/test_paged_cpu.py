@@ -85,3 +85,27 @@ def test_a_null_handle_gets_no_paged_cache():
     lib = _lib.load()
     assert lib.mk_batched_set_paged_cache(None, None) == _lib.MK_ERR_BAD_ARGUMENT
     assert b"null handle" in lib.mk_last_error()
+
+
+def test_attention_refuses_what_its_workspace_cannot_describe():
+    lib = _lib.load()
+    cache, batch, _, attention = good()
+    batch.seqs, batch.cu_tokens = 1025, 4096
+    assert lib.mk_paged_attention(cache, batch, attention, None) == _lib.MK_ERR_UNSUPPORTED
+    assert b"more sequences" in lib.mk_last_error()
+    cache, batch, _, attention = good()
+    cache.num_kv_heads = attention.num_q_heads = 0x8000
+    assert lib.mk_paged_attention(cache, batch, attention, None) == _lib.MK_ERR_UNSUPPORTED
+    assert b"KV heads" in lib.mk_last_error()
+
+
+def test_the_first_call_on_a_device_is_not_captured(monkeypatch):
+    monkeypatch.setattr(paged, "_error_words", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        paged._error_word(0)
+
+
+def test_a_cache_needs_room_for_a_position():
+    with pytest.raises(ValueError):
+        paged.PagedKvCache(1, 4, 1, 64, max_positions=0, device="cpu")

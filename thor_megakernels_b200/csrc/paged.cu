@@ -22,6 +22,8 @@ static int refuse(int code, const char *who, const char *text) {
     return code;
 }
 
+constexpr int kMaxKvHeads = 0x7fff;   // JoinEntry keeps a head in 16 bits
+
 static bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 // Pool and batch of a call, or an error code.
@@ -113,6 +115,7 @@ extern "C" int64_t mk_paged_attention_workspace(const MkPagedCache *cache, const
     int sms = 0;
     if (read_cache(*cache, *batch, MK_PAGED_ATTENTION_MAX_SEQS, pool, bt, who) || sm_count(sms)) return -1;
     if (num_q_heads < 1 || num_q_heads % pool.kv_heads) return refuse(MK_ERR_UNSUPPORTED, who, "query heads are not a multiple of the KV heads"), -1;
+    if (pool.kv_heads > kMaxKvHeads) return refuse(MK_ERR_UNSUPPORTED, who, "more KV heads than one call takes"), -1;
     const long long bytes = attention_workspace(bt, pool, num_q_heads, sms);
     if (bytes < 0) refuse(MK_ERR_UNSUPPORTED, who, "more rows times positions than one call takes");
     return bytes;
@@ -129,6 +132,7 @@ extern "C" int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch 
         return refuse(MK_ERR_BAD_ARGUMENT, who, "query or output rows null or not on 16-byte boundaries");
     if (a->num_q_heads < 1 || a->num_q_heads % pool.kv_heads)
         return refuse(MK_ERR_UNSUPPORTED, who, "query heads are not a multiple of the KV heads");
+    if (pool.kv_heads > kMaxKvHeads) return refuse(MK_ERR_UNSUPPORTED, who, "more KV heads than one call takes");
     if (!(fabsf(a->scale) <= 3.0e38f)) return refuse(MK_ERR_BAD_ARGUMENT, who, "scale is not finite");
     int sms = 0;
     code = sm_count(sms);

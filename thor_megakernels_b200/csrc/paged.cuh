@@ -51,7 +51,7 @@ __device__ __forceinline__ void rows_of(const Batch &bt, int b, int &first, int 
 
 // Cached length of sequence b, held inside its page table.
 __device__ __forceinline__ int length_of(const Batch &bt, int b) {
-    const int len = __ldg(bt.where + b) + bt.where_offset;
+    const long long len = (long long)__ldg(bt.where + b) + bt.where_offset;
     const int held = clamp_int(len, 0, clamp_int((long long)bt.max_pages << bt.page_shift, 0, 0x7fffffff));
     if (len > held) atomicOr(bt.error, kErrorIndex);
     return held;
@@ -211,6 +211,9 @@ __device__ __forceinline__ bool next_segment(const Batch &bt, int kv_heads, cons
     return false;
 }
 
+// Sum of two counts, held at the largest int.
+__device__ __forceinline__ int add_held(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
+
 // Fills prefix [seqs + 1] in shared memory with the units before each sequence of those that have between
 // min_count and max_count new rows, and sets up the CTA's walk.  All THREADS threads call it.
 template <int THREADS>
@@ -226,21 +229,28 @@ __device__ __forceinline__ void plan_walk(const Batch &bt, int kv_heads, const F
         const int length = length_of(bt, b);
         const int n = count < min_count || count > max_count ? 0 : sequence_units(length, count, group, cut, kv_heads);
         prefix[b + 1] = n;
-        sum += n;
+        sum = add_held(sum, n);
     }
     int incl = sum;
 #pragma unroll
     for (int off = 1; off < 32; off *= 2) {
         const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
+        if (lane >= off) incl = add_held(incl, v);
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int before = incl - sum;
-    for (int i = 0; i < warp; ++i) before += scan[i];
+    int before = incl - sum, total = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+        if (i == warp) before += total;
+        total = add_held(total, scan[i]);
+    }
+    // Row offsets that do not grow can give rows to many sequences at once, more than the host counted on: no work then.
+    const bool refused = total == 0x7fffffff;
+    if (refused && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
     for (int b = b0; b < b1; ++b) {
         before += prefix[b + 1];
-        prefix[b + 1] = before;
+        prefix[b + 1] = refused ? 0 : before;
     }
     if (threadIdx.x == 0) prefix[0] = 0;
     __syncthreads();

@@ -256,7 +256,7 @@ append_kernel(const AppendParams p) {
     int first, count;
     rows_of(bt, b, first, count);
     const int start = __ldg(bt.where + b);
-    if (start < 0) return;                                 // idle sequence
+    if (start < 0 || ordinal < 0) return;                  // idle sequence; offsets that do not grow
     const long long column = (long long)(start >> bt.page_shift) + ordinal;
     const long long page_begin = column << bt.page_shift;
     if (page_begin >= (long long)start + count) return;    // the sequence's rows end before this slot's page

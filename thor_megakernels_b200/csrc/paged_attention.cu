@@ -794,7 +794,7 @@ DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count,
     const long long joins = blocks * pool.kv_heads < g.ctas ? blocks * pool.kv_heads : g.ctas, turns = (sms + joins - 1) / joins;
     g.join_turns = (int)(turns < rows ? turns : rows);
     g.split = tiles > 1;
-    g.too_many = most > 0x7fffffffll;
+    g.too_many = most >= 0x7fffffffll;
     g.partial_floats = g.split ? (long long)g.ctas * 2 * rows * (pool.head_dim + 2) : 0;
     return g;
 }

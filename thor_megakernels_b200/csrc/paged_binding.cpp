@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <optional>
@@ -159,13 +160,21 @@ struct OnDevice {   // the device of a call as the current one, left alone where
 };
 void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
-PyObject *failed(const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
+// Whether two tensors' memory, from the first element to the last, overlaps.
+bool overlap(const at::Tensor &a, const at::Tensor &b) {
+    if (!a.numel() || !b.numel()) return false;
+    const auto bytes = [](const at::Tensor &t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return (last + 1) * (int64_t)t.element_size();
+    };
+    const char *pa = (const char *)a.const_data_ptr(), *pb = (const char *)b.const_data_ptr();
+    return pa < pb + bytes(b) && pb < pa + bytes(a);
 }
 
 // k, v, k_pages, v_pages, page_table, start, q, q_out, rope_cos, rope_sin, half_layout, k_scales, v_scales, cu_tokens
-PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) try {
+PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
     if (n != 14) return PyErr_Format(PyExc_TypeError, "append: %zd arguments", n);
     MkPagedCache c;
     MkPagedBatch b;
@@ -196,6 +205,11 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) try {
         if (!read_rows(*q, "q", -1, tokens, c.head_dim, device, args.q_token_stride, args.q_head_stride) ||
             !read_output(a[7], "q_out", *q, device, q_out))
             return nullptr;
+        if (a[7] != Py_None) {
+            const bool in_place = q_out.const_data_ptr() == q->const_data_ptr() && q->is_contiguous();
+            if (overlap(q_out, *k) || overlap(q_out, *v) || (!in_place && overlap(q_out, *q)))
+                return PyErr_Format(PyExc_ValueError, "q_out may be q itself, but overlap neither it in another way nor k or v");
+        }
         args.q = q->const_data_ptr();
         args.q_out = q_out.mutable_data_ptr();
         args.num_q_heads = (int32_t)q->size(1);
@@ -212,12 +226,12 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) try {
     }
     if (!q) Py_RETURN_NONE;
     return give(a[7], q_out);
-} catch (const std::exception &e) {
-    return failed(e);
+    END_HANDLE_TH_ERRORS
 }
 
 // q, k_pages, v_pages, page_table, lengths, scale, k_scales, v_scales, cu_tokens, out, workspace
-PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) try {
+PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
     if (n != 11) return PyErr_Format(PyExc_TypeError, "attention: %zd arguments", n);
     MkPagedCache c;
     MkPagedBatch b;
@@ -232,6 +246,7 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) try {
         return nullptr;
     const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)c.head_dim) : PyFloat_AsDouble(a[5]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    if (a[9] != Py_None && overlap(out, *q)) return PyErr_Format(PyExc_ValueError, "out must not overlap q");
     if (q->size(0) == 0) return give(a[9], out);
     if (!b.error_word) return PyLong_FromLong(-1);
     args.q = q->const_data_ptr();
@@ -254,12 +269,12 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) try {
     }
     if (const int code = g_attention(&c, &b, &args, stream_of(device))) return PyLong_FromLong(code);
     return give(a[9], out);
-} catch (const std::exception &e) {
-    return failed(e);
+    END_HANDLE_TH_ERRORS
 }
 
 // q, k_pages, v_pages, page_table, lengths, k_scales, v_scales, cu_tokens -> bytes as a float (an int is an error)
-PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) try {
+PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
     if (n != 8) return PyErr_Format(PyExc_TypeError, "attention_workspace: %zd arguments", n);
     MkPagedCache c;
     MkPagedBatch b;
@@ -275,8 +290,7 @@ PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) try 
     const int64_t bytes = g_workspace(&c, &b, (int32_t)q->size(1));
     if (bytes < 0) return PyLong_FromLong(MK_ERR_UNSUPPORTED);
     return PyFloat_FromDouble((double)bytes);
-} catch (const std::exception &e) {
-    return failed(e);
+    END_HANDLE_TH_ERRORS
 }
 
 // addresses of mk_paged_append, mk_paged_attention, mk_paged_attention_workspace

@@ -845,7 +845,7 @@ PrefillGrid prefill_grid(const Pool &pool, const Batch &bt, int hq, int min_coun
     const long long blocks = bt.cu ? (long long)bt.tokens * group / kBlockRows + bt.seqs : (long long)bt.seqs * block_count(bt.per_seq, group, kBlockRows);
     const long long tiles = (((long long)bt.max_pages << bt.page_shift) + kTileTokens - 1) / kTileTokens;
     const long long units = blocks * pool.kv_heads * (tiles + kPrefillCost);
-    g.too_many = units > 0x7fffffffll;
+    g.too_many = units >= 0x7fffffffll;
     g.ctas = g.too_many ? 0 : units < sms ? (int)units : sms;
     g.partial_floats = (long long)g.ctas * 2 * kBlockRows * (pool.head_dim + 2);
     return g;

@@ -57,7 +57,11 @@ def _binding():
 def _error_word(device: int) -> torch.Tensor:
     word = _error_words.get(device)
     if word is None:
+        # it outlives every graph, so it must not come from a graph's memory
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first paged call on a device cannot be captured in a CUDA graph: make one before (check_errors will do)")
         word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
+        torch.cuda.current_stream(device).synchronize()
         _binding().set_error_word(device, word.data_ptr())
         _error_words[device] = word
     return word
@@ -76,7 +80,8 @@ def _result(value, call, pages, args):
 def append(k, v, k_pages, v_pages, page_table, start, *, q=None, q_out=None, rope_cos=None, rope_sin=None, layout="interleaved",
            k_scales=None, v_scales=None, cu_tokens=None):
     """Store new key and value rows at positions ``start[b], start[b] + 1, ...`` of every sequence, keys (and
-    queries) rotated on the way.  Returns the rotated ``q`` (``q_out`` if given), or None without ``q``.
+    queries) rotated on the way.  Returns the rotated ``q`` (``q_out`` if given; it may be ``q`` itself), or None
+    without ``q``.
 
     ``start``: int32 ``[sequences]``; a negative one marks an idle sequence, whose rows are neither stored nor
     rotated.  ``rope_cos`` / ``rope_sin``: fp32 ``[positions, rot]`` tables, ``rot`` a multiple of 16 up to
@@ -100,9 +105,9 @@ def attention(q, k_pages, v_pages, page_table, lengths, *, scale=None, k_scales=
     ``[tokens, heads, head_dim]`` with heads a multiple of the cache's; returns ``out`` of the same shape, bf16.
 
     ``lengths``: int32 ``[sequences]``, the new rows included.  A row that sees no position (an idle sequence of
-    length 0) becomes zero; rows outside every sequence stay as they were in ``out``.  ``scale`` defaults to
-    ``1 / sqrt(head_dim)``.  ``workspace``: a uint8 tensor of ``attention_workspace`` bytes for callers that
-    allocate once; calls that may overlap in time need their own."""
+    length 0) becomes zero; rows outside every sequence stay as they were in ``out``, which must not overlap ``q``.
+    ``scale`` defaults to ``1 / sqrt(head_dim)``.  ``workspace``: a uint8 tensor of ``attention_workspace`` bytes for
+    callers that allocate once; calls that may overlap in time need their own."""
     call = _binding().attention
     args = (q, k_pages, v_pages, page_table, lengths, scale, k_scales, v_scales, cu_tokens, out, workspace)
     value = call(*args)
@@ -146,8 +151,8 @@ class PagedKvCache:
             raise ValueError(f"page_size must be one of {PAGE_SIZES} and head_dim one of {HEAD_DIMS}")
         if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError("the cache must be bf16 or float8_e4m3fn")
-        if min(num_layers, num_pages, num_kv_heads, max_seqs) < 1:
-            raise ValueError("layers, pages, heads and sequences must be positive")
+        if min(num_layers, num_pages, num_kv_heads, max_seqs, 1 if max_positions is None else max_positions) < 1:
+            raise ValueError("layers, pages, heads, sequences and positions must be positive")
         self.page_size, self.num_pages = page_size, num_pages
         shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
         # what a page holds before its first row is never read
@@ -157,6 +162,8 @@ class PagedKvCache:
             self.k_scales, self.v_scales = (torch.ones(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
         columns = num_pages if max_positions is None else -(-max_positions // page_size)
         self.page_table = torch.full((max_seqs, columns), -1, dtype=torch.int32, device=device)
+        if self.k.is_cuda:
+            _error_word(self.k.get_device())   # so that the first call may be a captured one
         self._free = list(range(num_pages - 1, -1, -1))
         self._owned: list[list[int]] = [[] for _ in range(max_seqs)]
 
