@@ -760,3 +760,29 @@ def test_a_captured_append_and_attention_follow_their_inputs(dtype):
         graph.replay()
         assert torch.equal(got, w)
     paged.check_errors()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_cache_layer_by_layer(dtype):
+    """A prompt, then single tokens of two of three sequences, through PagedKvCache.layer."""
+    from thor_megakernels_b200 import paged
+
+    gen = generator(49)
+    cache = paged.PagedKvCache(2, 20, 2, 64, page_size=16, max_seqs=3, max_positions=96, dtype=dtype)
+    lengths = [37, 16]
+    for b, n in enumerate(lengths):
+        cache.reserve(b, n + 2)
+    cu, start = ints([0, 37, 53]), ints([0, 0])
+    for new, at, offsets in ((53, start, cu), (2, ints(lengths), None), (2, ints([n + 1 for n in lengths]), None)):
+        seen = at + (ints(lengths) if offsets is not None else 1)
+        for layer in range(2):
+            k, v = (torch.randn((new, 2, 64), generator=gen, device="cuda").bfloat16() for _ in range(2))
+            q = torch.randn((new, 6, 64), generator=gen, device="cuda").bfloat16()
+            args = cache.layer(layer, 2)
+            paged.append(k, v, **args, start=at, cu_tokens=offsets)
+            got = paged.attention(q, **args, lengths=seen, cu_tokens=offsets)
+            paged.check_errors()
+            check_attention(got, q, args["k_pages"], args["v_pages"], args.get("k_scales"), args.get("v_scales"), args["page_table"], seen, offsets, 16, 1 / 8)
+    for b in range(2):
+        cache.release(b)
+    assert cache.free_pages == 20

@@ -197,10 +197,10 @@ class PagedKvCache:
         self._owned[seq] = []
         self.page_table[seq].fill_(-1)
 
-    def layer(self, index: int) -> dict:
-        """One layer's tensors as keyword arguments of ``append`` and ``attention``."""
+    def layer(self, index: int, seqs: int | None = None) -> dict:
+        """One layer's tensors, for the first ``seqs`` sequences or all, as keyword arguments of ``append`` and ``attention``."""
         scales = {} if self.k_scales is None else dict(k_scales=self.k_scales[index], v_scales=self.v_scales[index])
-        return dict(k_pages=self.k[index], v_pages=self.v[index], page_table=self.page_table, **scales)
+        return dict(k_pages=self.k[index], v_pages=self.v[index], page_table=self.page_table[:seqs], **scales)
 
     def describe(self) -> _lib.MkPagedModelCache:
         """The cache as ``mk_batched_set_paged_cache`` takes it."""
