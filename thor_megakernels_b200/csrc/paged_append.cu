@@ -278,13 +278,7 @@ append_kernel(const AppendParams p) {
             raw[it] = is_v ? load8<LIN>(p, p.v, (p.hq + hkv) * D, t, head, 8 * chunk) : load8<LIN>(p, p.k, p.hq * D, t, head, 8 * chunk);
         }
     }
-    if (page < 0) return;                                  // no page: nothing is kept
-    if (page >= bt.num_pages) {
-        if (threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
-        return;
-    }
     const bool rotated = rope && !is_v;
-    if (rotated && page_begin + end > p.positions && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
     const long long pos0 = page_begin + held;
     // row `it` of this thread in fp32, keys rotated
     auto value = [&](int it, float2 (&x)[4]) {
@@ -297,6 +291,17 @@ append_kernel(const AppendParams p) {
             widen(raw[it].x, x[0]); widen(raw[it].y, x[1]); widen(raw[it].z, x[2]); widen(raw[it].w, x[3]);
         }
     };
+    // the rows are made before the page id is looked at: the tables' elements arrive with it, not after it
+    float2 kept[ITERS][4];
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it)
+        if (it * kRows < added) value(it, kept[it]);
+    if (page < 0) return;                                  // no page: nothing is kept
+    if (page >= bt.num_pages) {
+        if (threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
+        return;
+    }
+    if (rotated && page_begin + end > p.positions && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
     const long long base = page * p.pool.page_stride + head * p.pool.head_stride + 8 * chunk;
     if constexpr (!FP8) {
         bf16 *dst = reinterpret_cast<bf16 *>(is_v ? p.pool.v : p.pool.k) + base;
@@ -304,18 +309,14 @@ append_kernel(const AppendParams p) {
         for (int it = 0; it < ITERS; ++it) {
             if (it * kRows < added) {
                 const int i = it * kRows + row_in_pass;
-                float2 x[4];
-                value(it, x);
-                if (i < added) *reinterpret_cast<uint4 *>(dst + (held + i) * p.pool.slot_stride) = round8(x);
+                if (i < added) *reinterpret_cast<uint4 *>(dst + (held + i) * p.pool.slot_stride) = round8(kept[it]);
             }
         }
     } else {
-        float2 kept[ITERS][4];
         float amax = 0.f;                                      // NaN never enters
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
             if (it * kRows < added) {
-                value(it, kept[it]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(kept[it][j].x), fabsf(kept[it][j].y)));
             }
