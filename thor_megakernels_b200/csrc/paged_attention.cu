@@ -648,19 +648,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     if (p.entries && threadIdx.x == 0) p.entries[blockIdx.x] = entry;
 }
 
-// Joins the parts of the segments that several CTAs shared: one CTA for the segment that begins in CTA
-// blockIdx.x's range, if there is one, and for a share of its rows.  A warp takes a row, or with fewer than
-// eight rows a share of a row's parts; its lanes read the statistics of 32 parts at once, then the parts one
-// after the other, D / 32 columns each.  The order of the sums is fixed.
+// Joins the parts of a segment that several CTAs shared, from CTA `from` on: this CTA's share of its rows.  A warp
+// takes a row, or with fewer than eight rows a share of a row's parts; its lanes read the statistics of 32 parts at
+// once, then the parts one after the other, D / 32 columns each.  The order of the sums is fixed.
 template <int D>
-__global__ void __launch_bounds__(256)
-join_kernel(const AttentionParams p, int rows_per_block) {
-    pdl_wait();   // and no early start for the next kernel: see paged.cuh
+__device__ __forceinline__ void join_segment(const AttentionParams &p, const JoinEntry &e, int from, int rows_per_block, float (&sum_o)[8][D],
+                                             float (&sum_m)[8], float (&sum_l)[8]) {
     constexpr int kCols = D / 32;
-    __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
-    const int4 raw = __ldg(reinterpret_cast<const int4 *>(p.entries + blockIdx.x));
-    const JoinEntry e = {raw.x, raw.y, raw.z, raw.w};
-    if (e.parts == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = e.head_rows & 0xffff, head = e.head_rows >> 16;
     const int share = (rows + gridDim.y - 1) / gridDim.y, row_end = min(rows, (int)(blockIdx.y + 1) * share);   // rows of this CTA
     const int per = share > 4 ? 1 : share > 2 ? 2 : share > 1 ? 4 : 8;                                          // warps per row
@@ -670,7 +664,7 @@ join_kernel(const AttentionParams p, int rows_per_block) {
 #pragma unroll
         for (int k = 0; k < kCols; ++k) O[k] = 0.f;
         auto part_of = [&](int i) {   // part i of the segment, this row
-            return p.partial + (((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
+            return p.partial + (((long long)(from + i) * 2 + (i == 0 ? 1 : 0)) * rows_per_block + r) * (D + 2);
         };
         if (r < row_end) {
             for (int base = sub; base < e.parts; base += 32 * per) {
@@ -731,19 +725,40 @@ join_kernel(const AttentionParams p, int rows_per_block) {
     }
 }
 
+// The segments that begin in the ranges of `entries` CTAs from blockIdx.x * entries on: few segments leave most
+// entries empty, and a CTA looks at 32 of them at once.
+template <int D>
+__global__ void __launch_bounds__(256)
+join_kernel(const AttentionParams p, int rows_per_block, int entries, int ctas) {
+    pdl_wait();   // and no early start for the next kernel: see paged.cuh
+    __shared__ float sum_o[8][D], sum_m[8], sum_l[8];
+    const int begin = blockIdx.x * entries, end = min(begin + entries, ctas), lane = threadIdx.x & 31;
+    for (int base = begin; base < end; base += 32) {
+        const int4 mine = base + lane < end ? __ldg(reinterpret_cast<const int4 *>(p.entries + base + lane)) : make_int4(0, 0, 0, 0);
+        for (unsigned todo = __ballot_sync(0xffffffffu, mine.x != 0); todo; todo &= todo - 1) {
+            const int l = __ffs(todo) - 1;
+            const JoinEntry e = {__shfl_sync(0xffffffffu, mine.x, l), __shfl_sync(0xffffffffu, mine.y, l), __shfl_sync(0xffffffffu, mine.z, l),
+                                 __shfl_sync(0xffffffffu, mine.w, l)};
+            join_segment<D>(p, e, base + l, rows_per_block, sum_o, sum_m, sum_l);
+            __syncthreads();   // the sums are the next segment's
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+
+// Query rows that a sequence of this call can have at most.
+static long long most_rows(const Batch &bt, int group, int max_count) {
+    return (long long)(bt.cu ? (bt.tokens < max_count ? bt.tokens : max_count) : bt.per_seq) * group;
+}
 
 // Tiles of 8 query rows per row block: one where no sequence of this call can have more rows, else two.  Four
 // would read the cache once for 17 to 32 rows, but their accumulators leave too few registers: 32 sequences x 5
 // tokens x 4 heads of a group against up to 16384 positions of E4M3, D = 128: one tile 256 us, two 187, four 294;
 // 16 x 5 x 4 against 4000 of bf16: 122, 86 and 108.  (12 rows: one tile 43.4, two 36.8.)
-static int row_tiles(const Batch &bt, int group, int max_count) {
-    const long long most = bt.cu ? (bt.tokens < max_count ? bt.tokens : max_count) : bt.per_seq;
-    const long long rows = most * group;
-    return rows <= 8 ? 1 : 2;
-}
+static int row_tiles(const Batch &bt, int group, int max_count) { return most_rows(bt, group, max_count) <= 8 ? 1 : 2; }
 
 bool make_pool_map(CUtensorMap *map, const Pool &pool, const void *base, int box_tokens, bool swizzle) {
     EncodeTiledFn fn = encode_tiled();
@@ -776,7 +791,9 @@ static int launch_decode_t(const AttentionParams &p, const Pool &pool, int sms, 
     if (e != cudaSuccess) return (int)e;
     const DecodeGrid grid = decode_grid(pool, p.bt, p.hq, p.max_count, sms);
     e = launch_pdl(decode_kernel<D, FP8, NT>, dim3(grid.ctas), dim3(kWarps * 32), smem, st, map_k, map_v, p);
-    if (e == cudaSuccess && grid.split) e = launch_pdl(join_kernel<D>, dim3(grid.ctas, grid.join_turns), dim3(256), 0, st, p, 8 * NT);
+    if (e == cudaSuccess && grid.split)
+        e = launch_pdl(join_kernel<D>, dim3((grid.ctas + grid.join_entries - 1) / grid.join_entries, grid.join_turns), dim3(256), 0, st, p,
+                       8 * NT, grid.join_entries, grid.ctas);
     return (int)e;
 }
 
@@ -798,7 +815,10 @@ DecodeGrid decode_grid(const Pool &pool, const Batch &bt, int hq, int max_count,
     g.ctas = (int)(most < resident ? most : resident);
     // segments to join: as many as there are row blocks, or CTAs where that is less; rows are dealt out until the GPU is full
     const long long joins = blocks * pool.kv_heads < g.ctas ? blocks * pool.kv_heads : g.ctas, turns = (sms + joins - 1) / joins;
-    g.join_turns = (int)(turns < rows ? turns : rows);
+    const long long held = most_rows(bt, group, max_count) < rows ? most_rows(bt, group, max_count) : rows;   // rows a block can have
+    g.join_turns = (int)(turns < held ? turns : held);
+    // few segments: their first CTAs lie ctas / joins apart, and CTAs of the join for every one between would only be launched
+    g.join_entries = g.ctas > 2 * joins ? (int)(g.ctas / (2 * joins)) : 1;
     g.split = tiles > 1;
     g.too_many = most >= 0x7fffffffll;
     g.partial_floats = g.split ? (long long)g.ctas * 2 * rows * (pool.head_dim + 2) : 0;

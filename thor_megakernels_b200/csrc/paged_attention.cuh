@@ -44,6 +44,7 @@ struct DecodeGrid {
     bool split;                     // a segment may be shared by several CTAs
     bool too_many;                  // more units than 32 bits count
     int join_turns;                 // CTAs that share a segment's rows in the join
+    int join_entries;               // CTAs of this kernel whose entries one of the join's looks at
     long long partial_floats;
 };
 
