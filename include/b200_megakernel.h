@@ -565,6 +565,9 @@ int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *batch, const 
  * and values): row i of n sees positions 0 .. length - n + i.  out = softmax(scale q k) v in
  * fp32, rounded once; rows that see nothing become zero, rows that belong to no
  * sequence are left as they were.  Query heads are a multiple of the KV heads.
+ * E4M3: scales are finite; a value scale below 2^-100 counts as 2^-100.  The value scale
+ * is part of the exponent the maximum runs over, so value scales that one row sees lie
+ * within a factor of 2^100: beyond it the weights of the smaller pages are lost.
  * The workspace (mk_paged_attention_workspace bytes for the same cache, batch sizes and
  * device; 16-byte aligned, contents irrelevant) must not be shared by calls that may
  * overlap in time.  Allocates nothing; may be captured in a CUDA graph.

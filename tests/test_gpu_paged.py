@@ -786,3 +786,21 @@ def test_a_cache_layer_by_layer(dtype):
     for b in range(2):
         cache.release(b)
     assert cache.free_pages == 20
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_value_scales_far_apart_and_zero(new):
+    """Equal scores over pages whose values are 2^90 apart: the denominator counts both; a scale of 0 makes a page of zeros."""
+    from thor_megakernels_b200 import paged
+
+    gen = generator(50)
+    k = torch.zeros((4, 1, 64, 64), device="cuda").to(FP8)
+    v = torch.randint(1, 5, (4, 1, 64, 64), generator=gen, device="cuda").float().to(FP8)
+    ks = torch.ones((4, 1), device="cuda")
+    q = torch.randn((new, 4, 64), generator=gen, device="cuda").bfloat16()
+    table, lengths = ints([[1, 3, 0]]), ints([192])
+    for scales in ([2.0 ** 60, 1.0, 9.0, 2.0 ** -30], [2.0, 1.0, 9.0, 0.0]):
+        vs = torch.tensor(scales, device="cuda").view(4, 1)
+        got = paged.attention(q, k, v, table, lengths, k_scales=ks, v_scales=vs)
+        paged.check_errors()
+        check_attention(got, q, k, v, ks, vs, table, lengths, None, 64, 1 / 8)

@@ -14,6 +14,7 @@ The functions take plain tensors:
   ``float8_e4m3fn``, last dimension dense, the others at any pitch that is a multiple of
   16 bytes (a dense cache ``[batch, positions, kv_heads, head_dim]`` seen as pages works).
 * ``k_scales`` / ``v_scales``: fp32 ``[pages, kv_heads]``, 8-bit caches only; a value is code times scale.
+  Finite; value scales that one row sees within a factor of 2^100 of one another.
 * ``page_table``: int32 ``[sequences, columns]``; a negative id means "no page".
 * token rows ``[tokens, heads, head_dim]`` bf16, last dimension dense.  Sequence ``b`` owns rows
   ``cu_tokens[b] .. cu_tokens[b + 1] - 1``, or ``tokens / sequences`` rows each without ``cu_tokens``.
