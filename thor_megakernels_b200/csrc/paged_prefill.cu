@@ -61,7 +61,6 @@ constexpr int kStepTokens = 64;            // positions of one product and softm
 constexpr int kBlockRows = 256;
 constexpr int kPanelBytes = 128 * 128;     // 128 rows of one 128-byte swizzle row
 constexpr int kChunks = kTileTokens / 16;  // a page is at least 16 positions
-constexpr int kBadBuffers = 4;
 constexpr float kLeastFactor = 1.17549435e-38f;   // of a score: minus infinity (a masked score) times it stays what it is
 
 // What the roles need of a segment besides its place.
@@ -91,6 +90,12 @@ struct Prefill {
     static constexpr int kRawTokens = kTileTokens / 2, kRawStages = FP8 ? 3 : 1;
     static constexpr int kRawBytes = FP8 ? kRawTokens * D : 16;
     static constexpr int kBadKinds = FP8 ? 1 : 3;                 // E4M3 has NaN only
+    // A tile-bearing segment's positions of values that are not finite, cleared by the loader when it comes to the segment and read
+    // last in its epilogue.  What the loader may run ahead of the epilogues, segments of one tile each: E4M3 codes of segment n - 1
+    // are all asked for once its first part is converted, so n - 2 is, for which the values' stage of n - 4 was free: that product
+    // is done, its epilogue may be under way, the one of n - 5 is over (queries are loaded behind it).  bf16: the keys' stage of
+    // n - 3 was free for n - 1, so the epilogue of n - 4 is over.
+    static constexpr int kBadBuffers = FP8 ? 5 : 4;
     struct __align__(1024) Smem {
         uint8_t q[2][kOperandBytes];
         uint8_t k[2][kOperandBytes];
@@ -404,7 +409,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             // epilogue
             if (n == 0) o_parity ^= 1u;   // a segment without steps counts one, so that this row tile is never ahead of it
             if (!(ok = wait_output(n > 0 ? (n - 1) & 1 : 0))) break;
-            const int buffer = bearing & (kBadBuffers - 1);
+            const int buffer = bearing % T::kBadBuffers;
             const bool bad = n > 0 && (volatile int &)s.bad_any[buffer] != 0;
             if (shape.most > 0) ++bearing;
             const bool complete = seg.begins && seg.ends;
@@ -472,7 +477,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         while (ok && advance_warp()) {
             const int n = shape.most;
             if (n == 0) continue;
-            const int buffer = bearing & (kBadBuffers - 1);
+            const int buffer = bearing % T::kBadBuffers;
             ++bearing;
             for (int c = lane; c < T::kBadKinds * D; c += 32) (&s.bad[buffer][0][0])[c] = 0x7fffffff;
             if (lane == 0) s.bad_any[buffer] = 0;
@@ -727,7 +732,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         while (ok && advance_warp()) {
             const int n = shape.most;
             if (n == 0) continue;
-            const int buffer = bearing & (kBadBuffers - 1);
+            const int buffer = bearing % T::kBadBuffers;
             ++bearing;
             for (int j = 0; ok && j < n; ++j, ++kv_it) {
                 const int pos0 = (seg.tile0 + j) * kTileTokens, stage = kv_it & 1;
@@ -868,6 +873,7 @@ static int launch_prefill_t(const PrefillParams &pp, const Pool &pool, const Pre
         set_last_error("mk_paged_attention: cuTensorMapEncodeTiled refused the cache (driver without tensor-map support?)");
         return MK_ERR_UNSUPPORTED;
     }
+    static_assert(offsetof(Smem, prefix) + (MK_PAGED_ATTENTION_MAX_SEQS + 1) * sizeof(int) <= 227 * 1024, "shared memory of a block");
     const size_t smem = offsetof(Smem, prefix) + (size_t)(pp.a.bt.seqs + 1) * sizeof(int);
     static bool allowed[64] = {};
     cudaError_t e = allow_smem((const void *)prefill_kernel<D, FP8>, allowed);
