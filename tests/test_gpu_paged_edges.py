@@ -65,3 +65,45 @@ def test_nan_in_the_causal_edge_of_many_short_prompts(dtype, tokens):
         assert torch.equal(torch.isnan(got), expect)
         assert torch.equal(got[~expect], clean[~expect])
     paged.check_errors()
+
+
+def peak_case(dtype, seqs, positions, new, gap, peak, kv_heads=1, group=4, dim=64, page=128):
+    """One position whose score stands `gap` above all others, which are alike, and whose values are zero: the result is what the
+    tail's weights make of its values.  Returns (call, reference in 64 bits, largest value)."""
+    gen = generator(positions + new)
+    pages = positions // page
+    k = torch.zeros((seqs * pages, kv_heads, page, dim), device="cuda")
+    v = torch.randint(1, 5, k.shape, generator=gen, device="cuda").float()
+    first = torch.arange(seqs, device="cuda") * pages + peak // page
+    k[first, :, peak % page, 0] = gap
+    v[first, :, peak % page] = 0
+    q = torch.zeros((seqs * new, kv_heads * group, dim), device="cuda")
+    q[..., 0] = 1
+    scales = dict(k_scales=torch.ones((seqs * pages, kv_heads), device="cuda"), v_scales=torch.ones((seqs * pages, kv_heads), device="cuda"))
+    table = torch.arange(seqs * pages, device="cuda").int().view(seqs, pages)
+    args = (q.bfloat16(), k.to(dtype), v.to(dtype), table, ints([positions] * seqs))
+    seen = positions - new + 1 + torch.arange(new, device="cuda")
+    tail = v.view(seqs, pages, kv_heads, page, dim).transpose(2, 3).reshape(seqs, positions, kv_heads, dim).double().cumsum(dim=1)[:, seen - 1]
+    there = (seen > peak).double()[None, :, None, None]
+    share = there * math.exp(-gap) + (1 - there)
+    want = tail * share / (there + (seen[None, :, None, None] - there) * share)
+    want = want.repeat_interleave(group, dim=2).reshape(q.shape)
+    return args, scales if dtype == FP8 else {}, want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [15, 16, 18, 20])
+@pytest.mark.parametrize("seqs,positions,new,kv_heads,peak", [(1, 65536, 1, 1, 77), (128, 4096, 1, 8, 1030), (128, 4096, 3, 8, 4090), (1, 65536, 512, 1, 65000),
+                                                              (32, 4096, 64, 8, 5), (32, 4096, 64, 8, 3000)])
+def test_a_peak_without_values_leaves_the_tail(dtype, gap, seqs, positions, new, kv_heads, peak):
+    """Rounding of the result 2^-8 and of a weight 2^-8 (bf16 pages, more than 32 rows per KV head) or 2^-11, scores and sums 2^-14;
+    E4M3 pages: an f16 weight loses at most half of 2^-24 below 2^11 times the largest, 2^-36 of the largest value a position."""
+    from thor_megakernels_b200 import paged
+
+    args, scales, want = peak_case(dtype, seqs, positions, new, gap, peak, kv_heads)
+    got = paged.attention(*args, scale=1.0, **scales)
+    paged.check_errors()
+    many = dtype == torch.bfloat16 and new * 4 > 32
+    tol = (2.0 ** -8 + (2.0 ** -8 if many else 2.0 ** -11) + 2.0 ** -14) * want + (positions * 2.0 ** -36 * 4 if dtype == FP8 else 0)
+    off = (got.double() - want).abs()
+    assert (off <= tol).all(), float((off / want).max())

@@ -25,8 +25,9 @@
 //     and two conversions give the fragment of even and odd columns.  Query rows enter as f16
 //     scaled by a power of two per row (exact for elements within 2^-31 of the row's largest).
 //   * The value scale joins the exponent: x + log2 vs is what the maximum runs over, so a weight
-//     that meets a page of large values is large in f16 and what is lost to its subnormals is
-//     small against the result.  The sum of the weights is taken in fp32 without that term.
+//     that meets a page of large values is large in f16.  f16 weights are scaled by 2^14: eleven
+//     bits down to 2^-28 of the largest, nothing below 2^-39, half of f16's smallest number.
+//     The sum of the weights is taken in fp32 without the value scale.
 //   * A bf16 cache keeps bf16 operands; a weight enters as two terms (value and remainder).
 //
 // Work split.  Units of (row block, KV head, tile of 4 warp tiles) are dealt to the resident
@@ -450,17 +451,17 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 #pragma unroll
                     for (int off = 4; off < 32; off *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                     const float mn = fmaxf(m[nt][e], mx);
-                    const float base = mn == -INFINITY ? 0.f : mn;
+                    const float base = mn == -INFINITY ? 0.f : mn, base_w = FP8 ? base - kFewWeight : base;
                     corr[nt][e] = exp2_fast(m[nt][e] - base);
                     rescale = rescale || mn != m[nt][e];
                     m[nt][e] = mn;
                     float add = 0.f;
 #pragma unroll
                     for (int mt = 0; mt < T::kMmaTiles; ++mt) {
-                        const float w0 = exp2_fast(sc[mt][nt][e] - base), w1 = exp2_fast(sc[mt][nt][2 + e] - base);
+                        const float w0 = exp2_fast(sc[mt][nt][e] - base_w), w1 = exp2_fast(sc[mt][nt][2 + e] - base_w);
                         sc[mt][nt][e] = w0;
                         sc[mt][nt][2 + e] = w1;
-                        add = fmaf(w0 + w1, inv_vs[mt], add);
+                        add = fmaf(FP8 ? (w0 + w1) * kFewUnscale : w0 + w1, inv_vs[mt], add);
                     }
                     l[nt][e] = fmaf(l[nt][e], corr[nt][e], add);
                 }
@@ -589,8 +590,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     for (int w = 0; w < kWarps; ++w) total = fmaf(sm.stat_l[w][r], exp2_fast(sm.stat_m[w][r] - base), total);
                     M[nt][e] = top;
                     L[nt][e] = total;
-                    f_own[nt][e] = exp2_fast(m[nt][e] - base);
-                    f_partner[nt][e] = exp2_fast(sm.stat_m[partner][r] - base);
+                    f_own[nt][e] = exp2_fast(m[nt][e] - base) * (FP8 ? kFewUnscale : 1.f);
+                    f_partner[nt][e] = exp2_fast(sm.stat_m[partner][r] - base) * (FP8 ? kFewUnscale : 1.f);
                 }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

@@ -11,6 +11,13 @@ namespace paged {
 constexpr int kWarps = 4;                          // warps per CTA of the few-row kernel
 constexpr long long kWaitCycles = 2000000000ll;    // limit of a wait, about a second
 
+// E4M3 pages: weights go to the tensor core as f16, times a power of two that uses the exponents above 1, so that what stands far
+// below the running maximum is not lost: its position may have small values, or none (sums of weights and results are divided by
+// it).  Without it a weight 17.4 (natural logarithm) below the maximum was gone from the numerator and still in the denominator.
+// Few rows: weights are at most 1 before it; prompts: at most 2^kPromptGrowth, the growth of the maximum that does not rescale.
+constexpr float kFewWeight = 14.f, kFewUnscale = 0x1p-14f;
+constexpr float kPromptGrowth = 4.f, kPromptWeight = 11.f, kPromptUnscale = 0x1p-11f;
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

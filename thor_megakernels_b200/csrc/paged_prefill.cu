@@ -13,8 +13,8 @@
 // instructions per warp.  To keep a row tile's threads from waiting for its products, S has two
 // buffers of 64 columns per row tile: while one step's weights are made, the next step's scores are there
 // already, and the one after takes the place of the weights as soon as their product is done.  The output is
-// rescaled only when the running maximum has grown by more than 2^8 since the last time (weights stay below
-// 256, sums are fp32), and only then do the softmax threads wait for the product before.
+// rescaled only when the running maximum has grown by more than 2^8 (E4M3: 2^4, its f16 weights are scaled by
+// 2^11 besides and stay below 2^15) since the last time (sums are fp32), and only then do the softmax threads wait for the product before.
 //
 // Warp roles: 0-3 and 4-7 softmax of row tile 0 and 1 (and query loading, epilogue), 8 loader (TMA,
 // one box per page), 9 and 10 MMA issue for one row tile each (9 also allocates tensor memory), 11 planner
@@ -85,6 +85,7 @@ struct Prefill {
     // (184 or 208 there: no faster).
     static constexpr int kSoftmaxRegisters = 200, kOtherRegisters = FP8 ? 56 : 104;
     static_assert(2 * kSoftmaxRegisters + (FP8 ? 2 : 1) * kOtherRegisters <= (FP8 ? 4 * 128 : 3 * 168), "within the launch's registers");
+    static constexpr float kGrowth = FP8 ? kPromptGrowth : 8.f;   // of the maximum that does not rescale the output
     static constexpr int kPanels = D / 64;
     static constexpr int kOperandBytes = kPanels * kPanelBytes;   // 128 rows x D two-byte elements
     static constexpr int kRawTokens = kTileTokens / 2, kRawStages = FP8 ? 3 : 1;
@@ -355,7 +356,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 // the running maximum, and the output if it has grown too much
                 {
                     const float grown = max3_nan(m, m, top);
-                    const bool need = !(grown <= m + 8.f);   // also from -inf, and NaN
+                    const bool need = !(grown <= m + T::kGrowth);   // also from -inf, and NaN
                     if (j == 0) {
                         m = grown;
                     } else if (__any_sync(0xffffffffu, need)) {
@@ -373,7 +374,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : m;
+                const float base = (m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : m) - (FP8 ? kPromptWeight : 0.f);
                 // weights, in the place of the scores
 #pragma unroll
                 for (int ch = 0; ch < 2; ++ch) {
@@ -394,7 +395,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                         float s0, s1;
                         split_f32(sum, s0, s1);
-                        l = fmaf(s0 + s1, s.iev[slot][4 * h + g], l);
+                        l = fmaf(FP8 ? (s0 + s1) * kPromptUnscale : s0 + s1, s.iev[slot][4 * h + g], l);
                     }
                     tmem_store16(s_h + 16 * ch, w);
                 }
@@ -413,7 +414,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const bool bad = n > 0 && (volatile int &)s.bad_any[buffer] != 0;
             if (shape.most > 0) ++bearing;
             const bool complete = seg.begins && seg.ends;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = l == 0.f ? 0.f : (FP8 ? kPromptUnscale : 1.f) / l;
             float *part = p.partial + ((long long)blockIdx.x * 2 + (seg.begins ? 1 : 0)) * kBlockRows * (D + 2);
             uint32_t x[D / 32][32];
             if (n > 0) {
@@ -837,7 +838,7 @@ join_blocks_kernel(const AttentionParams p) {
             sum[k].z = fmaf(sum[k].z, corr, v.z * f); sum[k].w = fmaf(sum[k].w, corr, v.w * f);
         }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float inv = total == 0.f ? 0.f : (p.k_scales ? kPromptUnscale : 1.f) / total;   // E4M3: the parts' outputs are scaled
     const int pair = e.pair + r;
     bf16 *dst = p.out + ((long long)(e.row + div(pair, p.group)) * p.hq + head * p.group.d + pair - div(pair, p.group) * p.group.d) * D + d0;
 #pragma unroll
