@@ -393,7 +393,8 @@ int mk_linear_batched_nvfp4(const void *w_packed, const void *w_scales_native, f
  *   tokens_out may be NULL.  Asynchronous on `stream`; allocates nothing, so it
  *   can be captured in a CUDA graph.  Token ids and positions are clamped on
  *   the device into [0, vocab) and [0, min(kv_max_len, rope_positions)) before
- *   anything indexes with them.
+ *   anything indexes with them.  (Over a paged cache positions are not clamped:
+ *   see mk_batched_set_paged_cache.)
  * mk_batched_status: synchronises `stream`; MK_ERR_DEVICE_WAIT if a bounded
  *   wait inside a linear ran out, MK_ERR_BAD_ARGUMENT if a token id or position
  *   had to be clamped since the last call.
@@ -590,9 +591,11 @@ int mk_paged_attention(const MkPagedCache *cache, const MkPagedBatch *batch, con
  * dense cache.  Layer l's pages and scales lie layer_stride elements and
  * scale_layer_stride floats behind layer 0's.  Sequence b (slot `slot` of a prefill)
  * owns row b of the page table; the caller puts pages there for every position before
- * the step that reaches it.  Positions are held below min(max_pages * page_size,
- * rope_positions); rows of a sequence without a page for them are not kept.  The
- * table and the pages are borrowed; NULL goes back to the dense cache.  Synchronises the
+ * the step that reaches it.  In a step a negative position marks an idle sequence:
+ * nothing of it is stored, its attention is zero and its logits and token mean nothing.
+ * A position at or beyond min(max_pages * page_size, rope_positions) makes its sequence
+ * idle too, and mk_batched_status reports it.  Rows of a sequence without a page for them
+ * are not kept.  The table and the pages are borrowed; NULL goes back to the dense cache.  Synchronises the
  * device and allocates the attention's workspace anew: CUDA graphs of earlier steps are void.
  */
 typedef struct MkPagedModelCache {

@@ -107,3 +107,42 @@ def test_a_peak_without_values_leaves_the_tail(dtype, gap, seqs, positions, new,
     tol = (2.0 ** -8 + (2.0 ** -8 if many else 2.0 ** -11) + 2.0 ** -14) * want + (positions * 2.0 ** -36 * 4 if dtype == FP8 else 0)
     off = (got.double() - want).abs()
     assert (off <= tol).all(), float((off / want).max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_with_idle_and_bad_positions_keeps_the_pages(dtype):
+    """Position -1: an idle slot.  A position beyond the cache: reported, and otherwise as idle.  Neither stores a row nor moves a
+    page's scale, and the sequences beside them get what they get without."""
+    from test_gpu_paged_decoder import build
+    from thor_megakernels_b200._lib import MegakernelError
+    from thor_megakernels_b200.batched import BatchedDecoder
+    from thor_megakernels_b200.paged import PagedKvCache
+
+    model = build(batch=4)
+    cache = PagedKvCache.for_model(model, 16, page_size=16, max_seqs=4, max_positions=64, dtype=dtype)
+    dec = BatchedDecoder(model, 4, cache=cache)
+    for b in range(4):
+        cache.reserve(b, 40)
+        dec.prefill(ints([3 + b, 50, 7, 11, 900 + b, 2, 31]), slot=b)
+    tensors = [t for t in (cache.k, cache.v, cache.k_scales, cache.v_scales) if t is not None]
+    kept = [t.clone() for t in tensors]
+    tokens = ints([5, 6, 7, 8])
+    dec.step(tokens, ints([7, 7, 7, 7]))
+    want = dec.logits[1].clone()
+    dec.status()
+    mine = cache.page_table[1, :3].long()
+    for bad, reported in (([-1, 7, -1, -5], False), ([-1, 7, 64, -2 ** 31], True), ([2 ** 31 - 1, 7, -1, 100], True)):
+        for t, k in zip(tensors, kept):
+            t.copy_(k)
+        dec.step(tokens, ints(bad))
+        if reported:
+            with pytest.raises(MegakernelError):
+                dec.status()
+        dec.status()
+        assert torch.equal(dec.logits[1], want)
+        assert torch.isfinite(dec.logits).all()
+        for t, k in zip(tensors, kept):
+            others = torch.ones(t.shape[1], dtype=torch.bool, device="cuda")
+            others[mine] = False
+            assert torch.equal(t[:, others].view(torch.uint8), k[:, others].view(torch.uint8))
+    dec.close()

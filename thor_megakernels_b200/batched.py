@@ -195,7 +195,9 @@ class BatchedDecoder:
 
     def step(self, tokens: torch.Tensor, pos_ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """``tokens`` and ``pos_ids``: int32 CUDA vectors of the same length
-        (``<= max_batch``).  Returns the greedy tokens (int32)."""
+        (``<= max_batch``).  Returns the greedy tokens (int32).  Over a paged cache
+        a negative position marks an idle slot: nothing is stored for it, and its
+        logits and token mean nothing."""
         for name, t in (("tokens", tokens), ("pos_ids", pos_ids)):
             if t.device.type != "cuda" or t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 CUDA vector")

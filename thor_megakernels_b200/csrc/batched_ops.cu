@@ -497,17 +497,19 @@ __global__ void fill_int_kernel(int *__restrict__ dst, int value, int step, int 
 // Positions arrive in device memory, where the host cannot look at them.  They are copied
 // into the handle's own array, clamped into [0, limit), so that no later kernel indexes
 // outside the rotary tables or the cache; a value that had to be clamped sets bit 1 of the
-// error word.
+// error word.  With `idle` (a paged cache) a value outside becomes -1 instead, which its append and
+// attention take for an idle sequence: a row at a place that nobody asked for can start a page's scale
+// afresh and spoil every row of the page.  Negative values ask for just that and are no error.
 __global__ void sanitize_positions_kernel(const int *__restrict__ pos_ids, int *__restrict__ pos_out, int batch, int pos_limit,
-                                          int *__restrict__ error) {
+                                          bool idle, int *__restrict__ error) {
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x * blockDim.x + threadIdx.x;
     if (b >= batch) return;
     const int q = pos_ids[b];
-    const int qc = q < 0 ? 0 : (q >= pos_limit ? pos_limit - 1 : q);
+    const int qc = q < 0 ? (idle ? -1 : 0) : q < pos_limit ? q : idle ? -1 : pos_limit - 1;
     pos_out[b] = qc;
-    if (qc != q) atomicOr(error, 2);
+    if (qc != q && !(idle && q < 0)) atomicOr(error, 2);
 }
 
 // Final values of the batched instruction set's dependency counters
@@ -537,9 +539,9 @@ __global__ void barrier_fill_kernel(int *__restrict__ barriers, const int *__res
 
 }  // namespace bo
 
-cudaError_t launch_sanitize_positions(const int *pos_ids, int *pos_out, int batch, int pos_limit, int *error, cudaStream_t st) {
+cudaError_t launch_sanitize_positions(const int *pos_ids, int *pos_out, int batch, int pos_limit, bool idle, int *error, cudaStream_t st) {
     return launch_pdl(bo::sanitize_positions_kernel, dim3((batch + 127) / 128), dim3(128), 0, st, pos_ids, pos_out, batch, pos_limit,
-                      error);
+                      idle, error);
 }
 
 cudaError_t launch_fill_int(int *dst, int value, int step, int n, cudaStream_t st) {

@@ -484,12 +484,12 @@ extern "C" int mk_step_batched(void *handle, const int32_t *tokens_in, const int
     const MkModelDesc &d = h->d;
     if (batch > (h->paged ? h->pg.seqs : d.kv_batch)) return fail_msg(MK_ERR_BAD_ARGUMENT, "mk_step_batched: the cache holds fewer sequences than the batch");
     Runner r;
-    // the kernels index with clamped copies of the caller's positions (bit 1 of the error word if any was out of range)
+    // the kernels index with copies of the caller's positions, clamped or (paged cache) idle where they are out of range, then bit 1 of the error word is set
     r.h = h; r.st = (cudaStream_t)stream; r.pos_ids = h->pos_uniform; r.rows = batch; r.half_split = 0; r.slice_down = 1;
     r.b = StepBuffers{(bf16 *)d.hidden_states, (bf16 *)d.logits, h->normed, h->normed, h->normed, h->q, h->attn, h->act,
                       (bf16 *)d.k_cache, (bf16 *)d.v_cache};
     r.use_pages = h->paged;
-    r.ok(launch_sanitize_positions(pos_ids, h->pos_uniform, batch, std::min(cache_positions(h), d.rope_positions), h->error_word, r.st));
+    r.ok(launch_sanitize_positions(pos_ids, h->pos_uniform, batch, std::min(cache_positions(h), d.rope_positions), h->paged, h->error_word, r.st));
     r.ok(launch_embed((const bf16 *)d.embed_w, tokens_in, r.b.hidden, batch, d.hidden_size, d.vocab_size, h->error_word, r.st));
     for (int l = 0; l < d.num_layers && r.code == 0; ++l) {
         r.attn_norm(l); r.qkv(l); r.attention(l); r.o_proj(l); r.mlp_norm(l); r.gate_up(l, true); r.down_proj(l);
@@ -697,7 +697,7 @@ extern "C" int mk_batched_status(void *handle, void *stream) {
     if (word != 0) {
         cudaMemset(h->error_word, 0, sizeof(int));
         if (word & 1) return fail_msg(MK_ERR_DEVICE_WAIT, "a bounded wait inside a batched linear ran out");
-        return fail_msg(MK_ERR_BAD_ARGUMENT, "a token id or position given to a batched step or prefill was outside the vocabulary / the cache and rotary tables (it was clamped), or a page id outside the paged cache (it was left out)");
+        return fail_msg(MK_ERR_BAD_ARGUMENT, "a token id or position given to a batched step or prefill was outside the vocabulary / the cache and rotary tables (it was clamped; over a paged cache a sequence with such a position was idle), or a page id outside the paged cache (it was left out)");
     }
     return 0;
 }
