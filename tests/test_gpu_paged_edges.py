@@ -146,3 +146,28 @@ def test_a_step_with_idle_and_bad_positions_keeps_the_pages(dtype):
             others[mine] = False
             assert torch.equal(t[:, others].view(torch.uint8), k[:, others].view(torch.uint8))
     dec.close()
+
+
+@pytest.mark.parametrize("new", [2, 5, 40])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_infinite_values_in_the_causal_edge(new, sign):
+    """bf16: the rows that see an infinite value are infinite in its column, not NaN; the others do not know of it."""
+    from thor_megakernels_b200 import paged
+
+    gen = generator(2)
+    k, v, _, _ = pool(torch.bfloat16, 8, 1, 32, 64, gen)
+    for length in (new, 33, 100, 190):
+        if length < new:
+            continue
+        w = v.clone()
+        at = length - 2
+        args = (ints([[6, 1, 4, 3, 0, 2]]), ints([length]))
+        q = torch.randn((new, 4, 64), generator=gen, device="cuda").bfloat16()
+        clean = paged.attention(q, k, v, *args)
+        w[int(args[0][0, at // 32]), 0, at % 32, 7] = sign * math.inf
+        got = paged.attention(q, k, w, *args)
+        assert torch.equal(got[:-2], clean[:-2])
+        assert (got[-2:, :, 7] == sign * math.inf).all()
+        keep = torch.arange(64, device="cuda") != 7
+        assert torch.equal(got[-2:][..., keep], clean[-2:][..., keep])
+    paged.check_errors()

@@ -452,7 +452,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                     for (int off = 4; off < 32; off *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                     const float mn = fmaxf(m[nt][e], mx);
                     const float base = mn == -INFINITY ? 0.f : mn, base_w = FP8 ? base - kFewWeight : base;
-                    corr[nt][e] = exp2_fast(m[nt][e] - base);
+                    // before the first score only an infinite value given by hand can be in the output: times 0 it would be NaN
+                    corr[nt][e] = !FP8 && m[nt][e] == -INFINITY ? 1.f : exp2_fast(m[nt][e] - base);
                     rescale = rescale || mn != m[nt][e];
                     m[nt][e] = mn;
                     float add = 0.f;
@@ -473,9 +474,12 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                         if constexpr (FP8) {
                             pf[mt][nt][h] = transpose8(pack_f16(w0, w1));
                         } else {
-                            const uint32_t hi = pack_b16(w0, w1);
+                            // cut off, not rounded, so that the remainder has the weight's sign, and kept above zero: an infinite
+                            // value times the two terms is infinite, not NaN (2^-126 is the least weight there is)
+                            const uint32_t hi = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x7632);
+                            const float r0 = fmaxf(w0 - bf16_lo(hi), fminf(w0, 0x1p-126f)), r1 = fmaxf(w1 - bf16_hi(hi), fminf(w1, 0x1p-126f));
                             pf[mt][nt][h] = transpose8(hi);
-                            pf_lo[mt][nt][h] = transpose8(pack_b16(w0 - bf16_lo(hi), w1 - bf16_hi(hi)));
+                            pf_lo[mt][nt][h] = transpose8(pack_b16(r0, r1));
                         }
                     }
                 }
