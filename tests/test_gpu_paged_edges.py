@@ -171,3 +171,21 @@ def test_infinite_values_in_the_causal_edge(new, sign):
         keep = torch.arange(64, device="cuda") != 7
         assert torch.equal(got[-2:][..., keep], clean[-2:][..., keep])
     paged.check_errors()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_rows_over_missing_pages_are_zero_whatever_the_queries_hold(dtype, new, what):
+    from thor_megakernels_b200 import paged
+
+    gen = generator(3)
+    k, v, ks, vs = pool(dtype, 8, 1, 32, 64, gen)
+    table, lengths = ints([[-1] * 6, [0, 1, 2, 3, 4, 5], [-1, -1, 6, 7, -1, -1]]), ints([150, 150, 150])
+    q = torch.randn((3 * new, 4, 64), generator=gen, device="cuda").bfloat16()
+    scales = dict(k_scales=ks, v_scales=vs)
+    clean = paged.attention(q, k, v, table, lengths, **scales)
+    q[:new] = what
+    got = paged.attention(q, k, v, table, lengths, **scales)
+    assert (got[:new] == 0).all() and torch.equal(got[new:], clean[new:])
+    paged.check_errors()

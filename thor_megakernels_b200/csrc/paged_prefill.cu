@@ -140,6 +140,17 @@ __device__ __forceinline__ Shape shape_of(const AttentionParams &p, const Segmen
     return h;
 }
 
+// Whether one of the positions below `limit` in a segment lies in a page of the pool.
+__device__ __forceinline__ bool any_page(const Batch &bt, const Segment &s, int limit) {
+    const int end = min(s.tile1 * kTileTokens, limit);
+#pragma unroll 1
+    for (int pos = s.tile0 * kTileTokens; pos < end; pos += 16) {
+        const int id = __ldg(bt.table + s.b * bt.table_stride + (pos >> bt.page_shift));
+        if (id >= 0 && id < bt.num_pages) return true;
+    }
+    return false;
+}
+
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *failed) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long began = clock64();
@@ -408,13 +419,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (!ok) break;
 
             // epilogue
+            if (l != l && !any_page(bt, seg, limit)) {   // a query that is not finite times the zeros of pages that are not there
+                m = -INFINITY;
+                l = 0.f;
+            }
             if (n == 0) o_parity ^= 1u;   // a segment without steps counts one, so that this row tile is never ahead of it
             if (!(ok = wait_output(n > 0 ? (n - 1) & 1 : 0))) break;
             const int buffer = bearing % T::kBadBuffers;
             const bool bad = n > 0 && (volatile int &)s.bad_any[buffer] != 0;
             if (shape.most > 0) ++bearing;
             const bool complete = seg.begins && seg.ends;
-            const float inv = l == 0.f ? 0.f : (FP8 ? kPromptUnscale : 1.f) / l;
             float *part = p.partial + ((long long)blockIdx.x * 2 + (seg.begins ? 1 : 0)) * kBlockRows * (D + 2);
             uint32_t x[D / 32][32];
             if (n > 0) {
@@ -424,6 +438,10 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                 for (int ch = 1; ch < D / 32; ++ch) after_wait(x[ch]);
             } else {
+#pragma unroll
+                for (int k = 0; k < D; ++k) x[k / 32][k % 32] = 0u;
+            }
+            if (l == 0.f) {   // nothing seen
 #pragma unroll
                 for (int k = 0; k < D; ++k) x[k / 32][k % 32] = 0u;
             }
@@ -439,6 +457,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     x[k / 32][k % 32] = __float_as_uint(y);
                 }
             }
+            const float inv = l == 0.f ? 0.f : (FP8 ? kPromptUnscale : 1.f) / l;
             if (complete) {   // through the query tile, which is idle now, to whole lines of the output
 #pragma unroll
                 for (int k = 0; k < D; k += 8) {
