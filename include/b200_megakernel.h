@@ -545,7 +545,8 @@ typedef struct MkPagedBatch {
  * of 16 up to head_dim; elements from rot_dim on pass unchanged; NULL: no rotation),
  * pairs (2i, 2i+1), or (i, i + rot_dim/2) with half_layout.  Products are rounded
  * separately in fp32, results once.  q / q_out may be NULL; rows of idle sequences
- * are left as they were.
+ * are left as they were.  With tables, rows at positions from rope_positions on are
+ * left out, keys, values and queries alike, and reported.
  *
  * E4M3: a page's scale is 2^e, e the smallest integer in [-64, 120] with
  * amax <= 448 * 2^e over the finite magnitudes of the page's rows; infinities

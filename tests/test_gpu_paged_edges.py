@@ -189,3 +189,35 @@ def test_rows_over_missing_pages_are_zero_whatever_the_queries_hold(dtype, new, 
     got = paged.attention(q, k, v, table, lengths, **scales)
     assert (got[:new] == 0).all() and torch.equal(got[new:], clean[new:])
     paged.check_errors()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,new", [(15, 10), (16, 9), (20, 3), (1000, 40), (0, 60), (19, 1), (20, 1)])
+def test_rows_beyond_the_rotary_tables_are_left_out(dtype, start, new):
+    """Tables of 20 positions: rows below are stored and rotated as if they came alone, those at or past the end are left out."""
+    from thor_megakernels_b200 import paged
+    from thor_megakernels_b200._lib import MegakernelError
+
+    gen = generator(4)
+    pages = 1200 // 16
+    a, b = (pool(dtype, pages, 2, 16, 64, generator(5)) for _ in range(2))
+    table = torch.arange(pages, device="cuda").int().view(1, pages)
+    rows = [torch.randn((new, h, 64), generator=gen, device="cuda").bfloat16() for h in (2, 2, 4)]
+    rows[0][-1] *= 1000   # would move a page's scale
+    rows[1][-1] *= 1000
+    angle = torch.rand((20, 32), generator=gen, device="cuda") * 6
+    tables = dict(rope_cos=angle.cos(), rope_sin=angle.sin(), layout="half")
+    outs = [torch.full_like(rows[2], 5.0) for _ in range(2)]
+    paged.append(rows[0], rows[1], a[0], a[1], table, ints([start]), q=rows[2], q_out=outs[0], k_scales=a[2], v_scales=a[3], **tables)
+    if start + new > 20:
+        with pytest.raises(MegakernelError):
+            paged.check_errors()
+    fits = max(0, min(new, 20 - start))
+    if fits:
+        paged.append(rows[0][:fits], rows[1][:fits], b[0], b[1], table, ints([start]), q=rows[2][:fits], q_out=outs[1][:fits], k_scales=b[2],
+                     v_scales=b[3], **tables)
+    paged.check_errors()
+    assert torch.equal(*outs)
+    for x, y in zip(a, b):
+        if x is not None:
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))

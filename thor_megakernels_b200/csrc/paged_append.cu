@@ -222,7 +222,10 @@ append_kernel(const AppendParams p) {
         if (rope) {
             const long long want = (long long)start + (t - first);
             const int pos = clamp_int(want, 0, p.positions - 1);
-            if (live && pos != want) atomicOr(bt.error, kErrorIndex);
+            if (live && pos != want) {                     // beyond the tables: left as it was
+                atomicOr(bt.error, kErrorIndex);
+                live = false;
+            }
             if (turn.inside) load_angles(p.rope_cos, p.rope_sin, (long long)pos * p.rot + 8 * chunk, turn, angles);
         }
         bf16 *dst = p.q_out + ((long long)t * p.hq + head0) * D + 8 * chunk;
@@ -259,17 +262,24 @@ append_kernel(const AppendParams p) {
     if (start < 0 || ordinal < 0) return;                  // idle sequence; offsets that do not grow
     const long long column = (long long)(start >> bt.page_shift) + ordinal;
     const long long page_begin = column << bt.page_shift;
-    if (page_begin >= (long long)start + count) return;    // the sequence's rows end before this slot's page
+    const long long past = (long long)start + count;       // the position behind the sequence's rows
+    if (page_begin >= past) return;                        // they end before this slot's page
     if (column >= bt.max_pages) {
         if (threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
         return;
     }
     const int held = page_begin < start ? (int)(start - page_begin) : 0;   // rows in the page before this call
-    const int end = (int)min((long long)page_size, (long long)start + count - page_begin);
+    // rows that the rotary tables do not reach, and their values, are left out
+    const long long stop = rope ? min(past, (long long)p.positions) : past;
+    const int end = (int)max(min((long long)page_size, stop - page_begin), 0ll);
     const int added = end - held;
     const int t0 = first + (int)(page_begin + held - start);               // token row of the page's first new row
 
     const int page = __ldg(bt.table + b * bt.table_stride + column);
+    if (stop < past && end < page_size) {
+        if (page >= 0 && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
+        if (added <= 0) return;
+    }
     uint4 raw[ITERS];
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
@@ -279,11 +289,11 @@ append_kernel(const AppendParams p) {
         }
     }
     const bool rotated = rope && !is_v;
-    const long long pos0 = page_begin + held;
+    const long long pos0 = page_begin + held;              // below p.positions where rows are rotated
     // row `it` of this thread in fp32, keys rotated
     auto value = [&](int it, float2 (&x)[4]) {
         if (rotated) {
-            const int pos = clamp_int(pos0 + min(it * kRows + row_in_pass, added - 1), 0, p.positions - 1);
+            const int pos = (int)pos0 + min(it * kRows + row_in_pass, added - 1);
             Angles angles;
             if (turn.inside) load_angles(p.rope_cos, p.rope_sin, (long long)pos * p.rot + 8 * chunk, turn, angles);
             rotate8(raw[it], angles, turn, x);
@@ -301,7 +311,6 @@ append_kernel(const AppendParams p) {
         if (threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
         return;
     }
-    if (rotated && page_begin + end > p.positions && threadIdx.x == 0) atomicOr(bt.error, kErrorIndex);
     const long long base = page * p.pool.page_stride + head * p.pool.head_stride + 8 * chunk;
     if constexpr (!FP8) {
         bf16 *dst = reinterpret_cast<bf16 *>(is_v ? p.pool.v : p.pool.k) + base;

@@ -87,7 +87,8 @@ def append(k, v, k_pages, v_pages, page_table, start, *, q=None, q_out=None, rop
     ``start``: int32 ``[sequences]``; a negative one marks an idle sequence, whose rows are neither stored nor
     rotated.  ``rope_cos`` / ``rope_sin``: fp32 ``[positions, rot]`` tables, ``rot`` a multiple of 16 up to
     ``head_dim`` (the rest of a head passes unchanged); ``layout`` "interleaved" pairs elements ``(2i, 2i + 1)``,
-    "half" pairs ``(i, i + rot / 2)``.  Without tables nothing is rotated.
+    "half" pairs ``(i, i + rot / 2)``.  Rows at positions beyond the tables are left out and reported.  Without
+    tables nothing is rotated.
 
     8-bit pages: see the module's header and ``mk_paged_append`` for how a page's scale is chosen and grows.
     Sequences of one call must not share the pages they append to."""
