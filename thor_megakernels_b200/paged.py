@@ -179,8 +179,13 @@ class PagedKvCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _check(self, seq: int) -> None:
+        if not 0 <= seq < len(self._owned):   # a negative index would be another sequence's
+            raise IndexError(f"the cache has sequences 0 .. {len(self._owned) - 1}, got {seq}")
+
     def reserve(self, seq: int, positions: int) -> None:
         """Give sequence ``seq`` pages for positions ``0 .. positions - 1`` (those it has stay its own)."""
+        self._check(seq)
         owned = self._owned[seq]
         need = -(-positions // self.page_size)
         if need > self.page_table.shape[1]:
@@ -195,6 +200,7 @@ class PagedKvCache:
 
     def release(self, seq: int) -> None:
         """Take all pages of sequence ``seq`` back."""
+        self._check(seq)
         self._free.extend(reversed(self._owned[seq]))
         self._owned[seq] = []
         self.page_table[seq].fill_(-1)
