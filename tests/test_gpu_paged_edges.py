@@ -221,3 +221,23 @@ def test_rows_beyond_the_rotary_tables_are_left_out(dtype, start, new):
     for x, y in zip(a, b):
         if x is not None:
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_reserve_and_release_do_not_wait_for_the_device():
+    """The table changes behind what is queued, and the host goes on."""
+    from thor_megakernels_b200 import paged
+
+    cache = paged.PagedKvCache(1, 8, 1, 64, page_size=16, max_seqs=3, max_positions=64)
+    cache.reserve(0, 5)   # the first pinned block is allocated
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)   # some 0.2 s of device time
+    cache.reserve(1, 30)
+    cache.reserve(2, 64)
+    cache.release(1)
+    cache.reserve(0, 40)
+    done.record()
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert cache.page_table.tolist() == [[0, 1, 2, -1], [-1] * 4, [3, 4, 5, 6]]
+    assert cache.free_pages == 1

@@ -19,3 +19,35 @@ def test_sequences_that_are_not_there_are_refused(seq):
     with pytest.raises(IndexError):
         c.release(seq)
     assert c.free_pages == 6 and torch.equal(c.page_table, before)
+
+
+def test_a_reserve_that_fails_costs_no_page(monkeypatch):
+    c = cache()
+    c.reserve(0, 20)
+    table = c.page_table.clone()
+
+    def fails(*args, **kw):
+        raise RuntimeError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "tensor", fails)
+        with pytest.raises(RuntimeError, match="no memory"):
+            c.reserve(1, 50)
+    assert c.free_pages == 6 and torch.equal(c.page_table, table)
+    c.reserve(1, 50)
+    assert c.free_pages == 2 and c.page_table[1].tolist() == [2, 3, 4, 5]
+
+
+def test_pages_are_handed_out_in_order_and_taken_back():
+    c = cache()
+    c.reserve(0, 17)
+    c.reserve(1, 1)
+    c.reserve(0, 33)
+    assert c.page_table.tolist() == [[0, 1, 3, -1], [2, -1, -1, -1], [-1] * 4]
+    c.release(0)
+    assert c.free_pages == 7 and c.page_table[0].tolist() == [-1] * 4
+    c.reserve(2, 64)
+    assert c.page_table[2].tolist() == [0, 1, 3, 4]
+    with pytest.raises(MemoryError):
+        c.reserve(0, 64)
+    assert c.free_pages == 3

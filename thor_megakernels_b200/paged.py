@@ -194,16 +194,19 @@ class PagedKvCache:
             return
         if need - len(owned) > len(self._free):
             raise MemoryError(f"{need - len(owned)} pages wanted, {len(self._free)} free")
-        new = [self._free.pop() for _ in range(need - len(owned))]
-        self.page_table[seq, len(owned):need] = torch.tensor(new, dtype=torch.int32, device=self.page_table.device)
+        new = self._free[len(owned) - need:][::-1]
+        # from pinned memory, which torch keeps until the copy is done: the host does not wait for what is queued
+        ids = torch.tensor(new, dtype=torch.int32, pin_memory=self.page_table.is_cuda)
+        self.page_table[seq, len(owned):need].copy_(ids, non_blocking=True)
+        del self._free[len(owned) - need:]   # only now: what raised above has cost no page
         owned.extend(new)
 
     def release(self, seq: int) -> None:
         """Take all pages of sequence ``seq`` back."""
         self._check(seq)
+        self.page_table[seq].fill_(-1)
         self._free.extend(reversed(self._owned[seq]))
         self._owned[seq] = []
-        self.page_table[seq].fill_(-1)
 
     def layer(self, index: int, seqs: int | None = None) -> dict:
         """One layer's tensors, for the first ``seqs`` sequences or all, as keyword arguments of ``append`` and ``attention``."""
