@@ -241,3 +241,22 @@ def test_reserve_and_release_do_not_wait_for_the_device():
     torch.cuda.synchronize()
     assert cache.page_table.tolist() == [[0, 1, 2, -1], [-1] * 4, [3, 4, 5, 6]]
     assert cache.free_pages == 1
+
+
+def test_pages_are_not_handed_out_inside_a_capture():
+    """The table would change with every replay and not now, the host's lists now and never again."""
+    from thor_megakernels_b200 import paged
+
+    cache = paged.PagedKvCache(1, 8, 1, 64, page_size=16, max_seqs=3, max_positions=64)
+    cache.reserve(0, 40)
+    before = cache.page_table.clone()
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.reserve(1, 20)
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.release(0)
+    graph.replay()
+    assert cache.free_pages == 5 and torch.equal(cache.page_table, before) and (x == 1).all()

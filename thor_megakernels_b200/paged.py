@@ -145,7 +145,7 @@ class PagedKvCache:
     (8-bit only), ``page_table`` int32 ``[max_seqs, max_pages]`` on the device, -1 where a sequence has no page.  A page id stands
     for the same place in every layer.  ``reserve`` before a call that reaches new positions, ``release`` when a sequence is done;
     both change the table in stream order (the current stream of the device), so a step that is queued already keeps its pages'
-    ids, and a captured step sees the table as it is when it is replayed."""
+    ids, and a captured step sees the table as it is when it is replayed.  Neither can be captured itself."""
 
     def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64, max_seqs: int = 128,
                  max_positions: int | None = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -182,6 +182,10 @@ class PagedKvCache:
     def _check(self, seq: int) -> None:
         if not 0 <= seq < len(self._owned):   # a negative index would be another sequence's
             raise IndexError(f"the cache has sequences 0 .. {len(self._owned) - 1}, got {seq}")
+        if self.page_table.is_cuda:
+            with torch.cuda.device(self.page_table.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("pages are handed out and taken back by the host: not inside a CUDA graph's capture")
 
     def reserve(self, seq: int, positions: int) -> None:
         """Give sequence ``seq`` pages for positions ``0 .. positions - 1`` (those it has stay its own)."""
