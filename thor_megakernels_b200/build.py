@@ -76,10 +76,23 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     return LIBRARY
 
 
+def binding_tag() -> str:
+    """What a ``_paged_binding.so`` has to be built from to be usable here: its source, the structs, torch's C++ and this
+    Python's C interface.  The module carries it as text."""
+    import hashlib
+    import sysconfig
+
+    import torch
+
+    text = b"".join(f.read_bytes() for f in (BINDING_SOURCE, PACKAGE_DIR.parent / "include" / "b200_megakernel.h"))
+    return f"mk_binding {hashlib.sha256(text).hexdigest()} torch {torch.__version__} {sysconfig.get_config_var('SOABI')};"
+
+
 def build_binding(force: bool = False) -> Path:
-    """Builds ``_paged_binding.so``, the CPython module behind ``paged`` (host code only, against the installed torch)."""
-    inputs = [BINDING_SOURCE, PACKAGE_DIR.parent / "include" / "b200_megakernel.h"]
-    if not force and BINDING.exists() and all(f.stat().st_mtime <= BINDING.stat().st_mtime for f in inputs):
+    """Builds ``_paged_binding.so``, the CPython module behind ``paged`` (host code only, against the installed torch), unless
+    the one that is there was built from the same."""
+    tag = binding_tag()
+    if not force and BINDING.exists() and tag.encode() in BINDING.read_bytes():
         return BINDING
     import sysconfig
 
@@ -90,6 +103,7 @@ def build_binding(force: bool = False) -> Path:
     scratch = BINDING.with_name(f"{BINDING.name}.{os.getpid()}.tmp")
     built = subprocess.run(
         ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+         f'-DMK_BINDING_TAG="{tag}"',
          "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
          "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"], str(BINDING_SOURCE), "-o", str(scratch),
          f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], capture_output=True, text=True)

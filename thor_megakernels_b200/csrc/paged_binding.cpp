@@ -293,9 +293,16 @@ PyObject *attention_workspace(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// addresses of mk_paged_append, mk_paged_attention, mk_paged_attention_workspace
+// What this module was built from; build.py looks for it in the file.
+__attribute__((used)) const char built_from[] = MK_BINDING_TAG;
+
+// addresses of mk_paged_append, mk_paged_attention, mk_paged_attention_workspace; the library's mk_abi_sizeof of the four structs
 PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (n != 3) return PyErr_Format(PyExc_TypeError, "init: %zd arguments", n);
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "init: %zd arguments", n);
+    const size_t sizes[4] = {sizeof(MkPagedCache), sizeof(MkPagedBatch), sizeof(MkPagedAppend), sizeof(MkPagedAttention)};
+    for (int i = 0; i < 4; ++i)
+        if (PyLong_AsLong(a[3 + i]) != (long)sizes[i])
+            return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_RuntimeError, "libb200mk.so and _paged_binding.so differ in their structs; build both anew");
     g_append = (AppendFn)PyLong_AsVoidPtr(a[0]);
     g_attention = (AttentionFn)PyLong_AsVoidPtr(a[1]);
     g_workspace = (WorkspaceFn)PyLong_AsVoidPtr(a[2]);

@@ -45,13 +45,14 @@ def _binding():
     lib = _lib.load()
     try:
         _build.build_binding()
-    except Exception as exc:  # no silent fallback
-        if not _build.BINDING.exists():
-            raise RuntimeError(f"_paged_binding.so is missing and could not be built ({exc}); run `python -m thor_megakernels_b200.build`") from exc
+    except Exception as exc:  # one built from other sources, or for another torch or Python, is not used
+        raise RuntimeError(f"_paged_binding.so is missing or of another build and could not be built ({exc}); "
+                           "run `python -m thor_megakernels_b200.build`") from exc
     from . import _paged_binding
 
     _paged_binding.init(*(C.cast(getattr(lib, name), C.c_void_p).value
-                          for name in ("mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace")))
+                          for name in ("mk_paged_append", "mk_paged_attention", "mk_paged_attention_workspace")),
+                        *(lib.mk_abi_sizeof(which) for which in (4, 5, 6, 7)))
     return _paged_binding
 
 
