@@ -198,7 +198,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
         }
     };
 
-    uint32_t stage = 0, parity = 0;   // the tile consumed next
+    uint32_t stage = 0, parity = 0;   // the tile consumed next (kStages: a wait ran out)
     uint32_t fill = 0;                // the stage filled next
     int in_flight = 0, odd = 0;       // filled stages; segments so far, mod 2
     JoinEntry entry = {0, 0, 0, 0};
@@ -216,6 +216,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     while (have) {
         int asked = ahead;   // tiles of this segment that have been asked for
         ahead = 0;
+        if (stage == T::kStages) mine.n = 0;
         while (in_flight < T::kStages && asked < mine.n && asked < 32) {
             issue(mine, cur.head, asked++, page_cur, fill);
             if (++fill == T::kStages) fill = 0;
@@ -322,12 +323,24 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 
             const uint32_t kt = ring + stage * 2 * T::kBytes, vt = kt + T::kBytes;
             const int pos0 = mine.from + i * T::kUnit;
-            if (!mbar_try_wait(&sm.full[warp][stage], parity)) {
-                const long long began = clock64();
-                bool ok;
-                while (!(ok = mbar_try_wait(&sm.full[warp][stage], parity)))
-                    if (clock64() - began > kWaitCycles) break;
-                if (!ok && lane == 0) atomicOr(bt.error, kErrorWait);
+            if (!__all_sync(0xffffffffu, mbar_try_wait(&sm.full[warp][stage], parity))) {
+                const auto wait = [&](uint64_t *bar, uint32_t par, long long began) {
+                    bool done;
+                    while (!(done = mbar_try_wait(bar, par)) && clock64() - began <= kWaitCycles) {}
+                    return done;
+                };
+                if (!__all_sync(0xffffffffu, wait(&sm.full[warp][stage], parity, clock64()))) {
+                    // The warp asks for no more tiles, here and in the segments to come, and does not leave with copies under way.
+                    if (lane == 0) atomicOr(bt.error, kErrorWait);
+                    const long long began = clock64();
+                    for (int k = 0; k < in_flight; ++k) {
+                        const RingFill f = ring_fill(stage, parity, k, T::kStages);
+                        wait(&sm.full[warp][f.stage], f.parity, began);
+                    }
+                    __syncwarp();
+                    stage = T::kStages;   // no stage: given up
+                    break;
+                }
             }
             __syncwarp();
 

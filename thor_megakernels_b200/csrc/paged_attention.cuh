@@ -46,6 +46,16 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
                  ::"r"(dst), "l"(map), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar)) : "memory");
 }
 
+// The fills of a ring that are under way, oldest first from the stage that is consumed next: stage of the k-th and parity of its
+// barrier.
+struct RingFill {
+    uint32_t stage, parity;
+};
+__host__ __device__ inline RingFill ring_fill(uint32_t stage, uint32_t parity, uint32_t k, uint32_t stages) {
+    const uint32_t s = stage + k;
+    return s < stages ? RingFill{s, parity} : RingFill{s - stages, parity ^ 1u};
+}
+
 struct DecodeGrid {
     int ctas;
     bool split;                     // a segment may be shared by several CTAs
