@@ -567,6 +567,7 @@ int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *batch, const 
  * and values): row i of n sees positions 0 .. length - n + i.  out = softmax(scale q k) v in
  * fp32, rounded once; rows that see nothing become zero, rows that belong to no
  * sequence are left as they were.  Query heads are a multiple of the KV heads.
+ * Positions from 2^31 - 65536 on count as outside the page table.
  * E4M3: scales are finite; a value scale below 2^-100 counts as 2^-100.  The value scale
  * is part of the exponent the maximum runs over, so value scales that one row sees lie
  * within a factor of 2^100: beyond it the weights of the smaller pages are lost.

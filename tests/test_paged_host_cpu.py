@@ -15,6 +15,13 @@ extern "C" void fill(uint32_t stage, uint32_t parity, uint32_t k, uint32_t stage
     out[0] = f.stage;
     out[1] = f.parity;
 }
+extern "C" int held(long long length, int max_pages, int page_shift) { return held_length(length, max_pages, page_shift); }
+extern "C" int tiles(int length, int count, int group, int rows, int rb, int tile) {
+    return block_tiles(length, count, fast_div(group), rows, rb, tile);
+}
+extern "C" int units(int length, int count, int group, int rows, int tile, int extra, int kv_heads) {
+    return sequence_units(length, count, fast_div(group), Cut{rows, tile, extra}, kv_heads);
+}
 """
 
 
@@ -46,3 +53,17 @@ def test_fills_under_way_are_found(host, stages):
             stage += 1
             if stage == stages:
                 stage, parity = 0, parity ^ 1
+
+
+@pytest.mark.parametrize("tile", [64, 128])
+@pytest.mark.parametrize("length", [1, 63, 64, 65, 2 ** 20, 2 ** 31 - 65537, 2 ** 31 - 65536, 2 ** 31 - 129, 2 ** 31 - 64, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 40])
+def test_lengths_up_to_the_largest_int(host, length, tile):
+    """A table of 2^24 pages of 128 holds more positions than an int counts: no length makes its tiles negative."""
+    host.held.argtypes = [C.c_longlong, C.c_int, C.c_int]
+    held = host.held(length, 2 ** 24 + 3, 7)
+    assert held == min(length, 2 ** 31 - 65536)
+    want = -(-held // tile)
+    assert host.tiles(held, 1, 4, 8, 0, tile) == want
+    assert host.units(held, 1, 4, 8, tile, 1, 8) == 8 * (want + 1)
+    assert host.held(length, 10, 4) == min(length, 160)
+    assert host.held(-length, 10, 4) == 0

@@ -49,10 +49,17 @@ __device__ __forceinline__ void rows_of(const Batch &bt, int b, int &first, int 
     if (first != lo || first + count != hi) atomicOr(bt.error, kErrorIndex);
 }
 
+// Most positions of a sequence that attention counts: the position behind any tile that is looked ahead to is an int.
+constexpr int kMostPositions = 0x7fff0000;
+
+__host__ __device__ inline int held_length(long long length, int max_pages, int page_shift) {
+    return clamp_int(length, 0, clamp_int((long long)max_pages << page_shift, 0, kMostPositions));
+}
+
 // Cached length of sequence b, held inside its page table.
 __device__ __forceinline__ int length_of(const Batch &bt, int b) {
     const long long len = (long long)__ldg(bt.where + b) + bt.where_offset;
-    const int held = clamp_int(len, 0, clamp_int((long long)bt.max_pages << bt.page_shift, 0, 0x7fffffff));
+    const int held = held_length(len, bt.max_pages, bt.page_shift);
     if (len > held) atomicOr(bt.error, kErrorIndex);
     return held;
 }
