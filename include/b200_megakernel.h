@@ -546,7 +546,8 @@ typedef struct MkPagedBatch {
  * pairs (2i, 2i+1), or (i, i + rot_dim/2) with half_layout.  Products are rounded
  * separately in fp32, results once.  q / q_out may be NULL; rows of idle sequences
  * are left as they were.  With tables, rows at positions from rope_positions on are
- * left out, keys, values and queries alike, and reported.
+ * left out, keys, values and queries alike, and reported.  Keys and values have pages
+ * and scales of their own, and no input row lies in a page that the call stores into.
  *
  * E4M3: a page's scale is 2^e, e the smallest integer in [-64, 120] with
  * amax <= 448 * 2^e over the finite magnitudes of the page's rows; infinities

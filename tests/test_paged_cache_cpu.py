@@ -51,3 +51,18 @@ def test_pages_are_handed_out_in_order_and_taken_back():
     with pytest.raises(MemoryError):
         c.reserve(0, 64)
     assert c.free_pages == 3
+
+
+def test_append_refuses_keys_and_values_in_the_same_pages():
+    """Both would be written by blocks of their own, in any order."""
+    from test_paged_cpu import good
+
+    from thor_megakernels_b200 import _lib
+
+    lib = _lib.load()
+    for changes in (dict(v_pages=4096), dict(format=_lib.MK_CACHE_E4M3, k_scales=4096, v_scales=4096)):
+        cache, batch, append, _ = good()
+        for name, value in changes.items():
+            setattr(cache, name, value)
+        assert lib.mk_paged_append(cache, batch, append, None) == _lib.MK_ERR_BAD_ARGUMENT
+        assert b"of their own" in lib.mk_last_error()

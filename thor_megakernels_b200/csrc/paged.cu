@@ -85,6 +85,8 @@ extern "C" int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *ba
     AppendParams p = {};
     int code = read_cache(*cache, *batch, MK_PAGED_MAX_SEQS, p.pool, p.bt, who);
     if (code) return code;
+    if (cache->k_pages == cache->v_pages || (p.pool.fp8 && cache->k_scales == cache->v_scales))
+        return refuse(MK_ERR_BAD_ARGUMENT, who, "keys and values need pages and scales of their own");
     if (bad_rows(a->k, a->k_token_stride, a->k_head_stride) || bad_rows(a->v, a->v_token_stride, a->v_head_stride))
         return refuse(MK_ERR_BAD_ARGUMENT, who, "key or value rows null or not on 16-byte boundaries");
     if ((a->q == nullptr) != (a->q_out == nullptr)) return refuse(MK_ERR_BAD_ARGUMENT, who, "q and q_out go together");
