@@ -66,3 +66,29 @@ def test_append_refuses_keys_and_values_in_the_same_pages():
             setattr(cache, name, value)
         assert lib.mk_paged_append(cache, batch, append, None) == _lib.MK_ERR_BAD_ARGUMENT
         assert b"of their own" in lib.mk_last_error()
+
+
+@pytest.mark.parametrize("value,code", [(1, "MK_ERR_DEVICE_WAIT"), (2, "MK_ERR_BAD_ARGUMENT"), (0, None)])
+def test_an_error_is_wiped_out_before_the_next_call_can_report(monkeypatch, value, code):
+    from thor_megakernels_b200 import _lib
+
+    log = []
+
+    class Word:
+        def item(self):
+            log.append("read")
+            return value
+
+        def zero_(self):
+            log.append("zero")
+
+    monkeypatch.setattr(paged, "_error_word", lambda device: Word())
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: log.append("sync"))
+    if code is None:
+        paged.check_errors("cuda:0")
+        assert log == ["sync", "read"]
+        return
+    with pytest.raises(_lib.MegakernelError) as raised:
+        paged.check_errors("cuda:0")
+    assert raised.value.code == getattr(_lib, code)
+    assert log == ["sync", "read", "zero", "sync"]

@@ -134,6 +134,7 @@ def check_errors(device=None) -> None:
     value = int(word.item())
     if value:
         word.zero_()
+        torch.cuda.synchronize(index)   # or it could wipe out what a later call on another stream reports
         if value & 1:
             raise _lib.MegakernelError(_lib.MK_ERR_DEVICE_WAIT, "a bounded wait inside a kernel ran out")
         raise _lib.MegakernelError(_lib.MK_ERR_BAD_ARGUMENT, "a page id, position, length or row offset given to a paged call was outside its tensor; it was left out")
