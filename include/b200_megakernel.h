@@ -565,11 +565,17 @@ int mk_paged_append(const MkPagedCache *cache, const MkPagedBatch *batch, const 
 
 /*
  * Causal attention of the new rows over the cache (which already holds their keys
- * and values): row i of n sees positions 0 .. length - n + i.  out = softmax(scale q k) v in
- * fp32, rounded once; rows that see nothing become zero, rows that belong to no
- * sequence are left as they were.  Query heads are a multiple of the KV heads.
- * Positions from 2^31 - 65536 on count as outside the page table.
- * E4M3: scales are finite; a value scale below 2^-100 counts as 2^-100.  The value scale
+ * and values): row i of n sees positions 0 .. length - n + i.  out = softmax(scale q k) v;
+ * rows that see nothing become zero, rows that belong to no sequence are left as they
+ * were.  Query heads are a multiple of the KV heads.  Positions from 2^31 - 65536 on
+ * count as outside the page table.
+ * Scores, softmax statistics and sums are held in fp32 and the result is rounded once.
+ * The softmax weights enter the second product rounded: over bf16 pages as two bf16 terms
+ * (2^-16 of themselves) where a sequence has at most 32 (new row, query head of a KV head)
+ * pairs, as one (2^-8) where it has more; over E4M3 pages as f16 (2^-11; with fewer bits
+ * below 2^-28 of the largest weight so far, 2^-25 with more than 32 pairs, and as zero
+ * below 2^-39 and 2^-36).
+ * E4M3: scales are finite and not negative; a value scale below 2^-100 counts as 2^-100.  The value scale
  * is part of the exponent the maximum runs over, so value scales that one row sees lie
  * within a factor of 2^100: beyond it the weights of the smaller pages are lost.
  * The workspace (mk_paged_attention_workspace bytes for the same cache, batch sizes and

@@ -260,3 +260,26 @@ def test_pages_are_not_handed_out_inside_a_capture():
             cache.release(0)
     graph.replay()
     assert cache.free_pages == 5 and torch.equal(cache.page_table, before) and (x == 1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_most_sequences_of_a_call(dtype):
+    """1024 ragged sequences, a few of them prompts, D = 128: both kernels with their largest lists of sequences."""
+    from thor_megakernels_b200 import paged
+
+    gen = generator(6)
+    seqs, page = 1024, 16
+    new = [(0, 1, 3)[b % 3] if b % 128 != 5 else 40 for b in range(seqs)]
+    lengths = [n + (7 * b) % 50 for b, n in enumerate(new)]
+    k, v, ks, vs = pool(dtype, seqs * 6, 1, page, 128, gen)
+    table = torch.randperm(seqs * 6, generator=gen, device="cuda").int().view(seqs, 6)
+    cu = ints([0] + list(torch.tensor(new).cumsum(0)))
+    q = torch.randn((sum(new), 2, 128), generator=gen, device="cuda").bfloat16()
+    got = paged.attention(q, k, v, table, ints(lengths), k_scales=ks, v_scales=vs, cu_tokens=cu)
+    paged.check_errors()
+    kd, vd = po.dequantise(k, ks), po.dequantise(v, vs)
+    want, mag = po.attention(q, kd, vd, table, ints(lengths), cu, page, 1 / math.sqrt(128))
+    tol = po.attention_tolerance(want, mag, dtype == FP8, 90, float(vd.abs().max()), True)
+    assert not torch.isnan(got).any() and ((got.double() - want).abs() <= tol).all()
+    with pytest.raises(Exception, match="more sequences"):
+        paged.attention(q, k, v, table.repeat(2, 1)[:1025], ints(lengths + [0]), k_scales=ks, v_scales=vs, cu_tokens=torch.cat((cu, cu[-1:])))

@@ -14,12 +14,12 @@ The functions take plain tensors:
   ``float8_e4m3fn``, last dimension dense, the others at any pitch that is a multiple of
   16 bytes (a dense cache ``[batch, positions, kv_heads, head_dim]`` seen as pages works).
 * ``k_scales`` / ``v_scales``: fp32 ``[pages, kv_heads]``, 8-bit caches only; a value is code times scale.
-  Finite; value scales that one row sees within a factor of 2^100 of one another.
+  Finite and not negative; value scales that one row sees within a factor of 2^100 of one another.
 * ``page_table``: int32 ``[sequences, columns]``; a negative id means "no page".
 * token rows ``[tokens, heads, head_dim]`` bf16, last dimension dense.  Sequence ``b`` owns rows
   ``cu_tokens[b] .. cu_tokens[b + 1] - 1``, or ``tokens / sequences`` rows each without ``cu_tokens``.
 
-Nothing synchronises.  Page ids, positions and offsets live on the device and are checked there:
+For inference: results carry no gradient.  Nothing synchronises.  Page ids, positions and offsets live on the device and are checked there:
 what lies outside its tensor is left out, and the next ``check_errors`` raises.
 """
 from __future__ import annotations
@@ -109,6 +109,7 @@ def attention(q, k_pages, v_pages, page_table, lengths, *, scale=None, k_scales=
 
     ``lengths``: int32 ``[sequences]``, the new rows included.  A row that sees no position (an idle sequence of
     length 0) becomes zero; rows outside every sequence stay as they were in ``out``, which must not overlap ``q``.
+    Scores, statistics and sums are fp32; how the softmax weights are rounded stands at ``mk_paged_attention``.
     ``scale`` defaults to ``1 / sqrt(head_dim)``.  ``workspace``: a uint8 tensor of ``attention_workspace`` bytes for
     callers that allocate once; calls that may overlap in time need their own."""
     call = _binding().attention
