@@ -37,7 +37,7 @@
 // segment's first tiles are requested before the last one's merge.
 //
 // Measured (device time of this kernel + the join, one token each, 32 query and 8 KV heads, D = 128): 128 sequences
-// of 512 to 4096 positions, E4M3, 600 MB: 108 + 4 us, 5.4 TB/s, HBM-bound; 17 sequences of them in bf16, 167 MB:
+// of 512 to 4096 positions, E4M3, 600 MB: 105 + 4 us, 5.5 TB/s, HBM-bound; 17 sequences of them in bf16, 167 MB:
 // 32 + 5 us; one of 65521, E4M3, 134 MB: 30 + 7 us.  The shorter the call, the more of it are the start (planning,
 // first tiles: some 4 us) and the join; 115 positions take 5.3 us.
 

@@ -24,7 +24,7 @@
 // and the value scale joins the exponent, as in paged_attention.cu.  A bf16 cache goes from TMA
 // to the tensor core without passing a register; its weights are one bf16 term each (2^-8 of a weight, what the
 // result's own rounding is: 4 prompts are 0.0017 of their norm off the 64-bit result, 0.0015 with fp32 weights; a second
-// term would be half a score's tensor work more and a longer chain).
+// term would be half of the tensor work more and a longer chain).
 //
 // Values that are not finite and lie at positions some rows do not see (or behind the end) are
 // taken out of the tile by the warp that fills it; rows that do see them get them in the epilogue.
@@ -34,8 +34,8 @@
 // Row blocks that a range's end cuts are joined by a second kernel.
 //
 // Measured (device time of this kernel + the join): 4 prompts of 333 to 3001 rows, bf16, 32 query and 8 KV heads,
-// D = 128: 238 + 11 us, 0.75 PFLOP/s; 512 rows behind 8192 positions, E4M3: 95 + 8 us, 0.75 PFLOP/s.  The tensor
-// pipe is busy for 38 % of the cycles and the special function unit as long: a row tile's step is one chain (scores
+// D = 128: 244 + 11 us, 0.73 PFLOP/s; 512 rows behind 8192 positions, E4M3: 99 + 8 us, 0.72 PFLOP/s.  The tensor
+// pipe is busy for 35 to 37 % of the cycles and the special function unit as long: a row tile's step is one chain (scores
 // from tensor memory, maximum, exponentials, weights to tensor memory, product), and two row tiles x two steps in
 // flight do not fill the pipes between its parts.
 
