@@ -524,8 +524,8 @@ typedef struct MkPagedCache {
  * negative page id means "no page": nothing is stored there, and its positions
  * take no part in attention.  Page ids, positions and row offsets are device data
  * and are checked there: what lies outside its tensor is left out and bit 1 (value
- * 2) of *error_word is set; bit 0 if a bounded wait ran out.  Sequences of one call
- * do not share the pages that it stores into.
+ * 2) of *error_word is set; bit 0 if a bounded wait ran out.  The pages that a call
+ * stores into are shared neither between its sequences nor within one.
  */
 typedef struct MkPagedBatch {
     const int32_t *page_table;     /* device [seqs, max_pages], rows table_stride apart */

@@ -92,7 +92,7 @@ def append(k, v, k_pages, v_pages, page_table, start, *, q=None, q_out=None, rop
     tables nothing is rotated.
 
     8-bit pages: see the module's header and ``mk_paged_append`` for how a page's scale is chosen and grows.
-    Sequences of one call must not share the pages they append to."""
+    A page that a call appends to must stand in one place of the sequences' tables only."""
     if layout != "interleaved" and layout != "half":
         raise ValueError(f"layout must be 'interleaved' or 'half', got {layout!r}")
     call = _binding().append
